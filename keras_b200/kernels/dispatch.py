@@ -369,6 +369,22 @@ def flash_attention(q, k, v, mask, scale, is_causal, row_mask=None):
     return attention.flash_attention(q, k, v, mask, scale, is_causal, row_mask)
 
 
+def rule_attention(q, k, v, rules, plain):
+    if not enabled(q):
+        return None
+    from keras_b200.kernels import attention_rules
+
+    return attention_rules.attention(q, k, v, rules, plain)
+
+
+def cached_attention(q, k, v, pool_k, pool_v, pages, lengths, rules):
+    if not enabled(q):
+        return None
+    from keras_b200.kernels import attention_cache
+
+    return attention_cache.attention(q, k, v, pool_k, pool_v, pages, lengths, rules.scale, rules.cap, rules.slopes, rules.window)
+
+
 # ---------------------------------------------------------------------------- recurrent layers
 def lstm_takes(sequences, initial_state, cell):
     """Whether the whole-sequence kernel runs this LSTM layer: float32 CUDA tensors, unsharded weights, a size it takes."""

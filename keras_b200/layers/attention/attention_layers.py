@@ -19,6 +19,7 @@ from keras_b200.layers.activations.activation_layers import Softmax
 from keras_b200.layers.core.einsum_dense import EinsumDense
 from keras_b200.layers.layer import Layer
 from keras_b200.layers.regularization.regularization_layers import Dropout
+from keras_b200.ops import attention_rules
 
 _LETTERS = string.ascii_lowercase
 
@@ -60,11 +61,81 @@ def _full_shape(rank, last):
     return [None] * (rank - len(last)) + list(last)
 
 
+def _fixed_rules(layer, attn_logits_soft_cap, distance_slopes, heads, dropout):
+    """Sets a layer's rules that every call follows (``ops.dot_product_attention`` says what they do)."""
+    layer._attn_logits_soft_cap = None if attn_logits_soft_cap is None else attention_rules.soft_cap(attn_logits_soft_cap)
+    if distance_slopes is not None:
+        distance_slopes = tuple(float(s) for s in distance_slopes)
+        if len(distance_slopes) != heads:
+            raise ValueError(f"`distance_slopes` has to hold one number a query head ({heads}). Received: distance_slopes={distance_slopes}")
+    layer._distance_slopes = distance_slopes
+    layer.__dict__["_slopes_on"] = {}  # not tracked: made again where it is needed
+    if dropout > 0.0 and (attn_logits_soft_cap is not None or distance_slopes is not None):
+        raise ValueError("Dropout is not supported with `attn_logits_soft_cap` or `distance_slopes`. Please set dropout to 0.0.")
+
+
+def _rules_config(layer):
+    """Entries of the configuration that say rules; none for a layer without."""
+    given = {"attn_logits_soft_cap": layer._attn_logits_soft_cap, "distance_slopes": None if layer._distance_slopes is None else list(layer._distance_slopes)}
+    return {k: v for k, v in given.items() if v is not None}
+
+
+def _slopes_of(layer, like):
+    """The layer's slopes on the device of a tensor: made once a device, so that a recorded step copies nothing from the host."""
+    if layer._distance_slopes is None:
+        return None
+    if not isinstance(like, torch.Tensor) or like.device.type == "meta":
+        return list(layer._distance_slopes)
+    on = layer._slopes_on.get(like.device)
+    if on is None:
+        on = layer._slopes_on[like.device] = torch.tensor(layer._distance_slopes, dtype=torch.float32, device=like.device)
+    return on
+
+
+def _attend_by_rules(layer, q, k, v, scale, masks, use_causal_mask, return_attention_scores, dropout, segment_ids, prefix_lengths, cache, sharded):
+    """The attention of a call that has rules or a cache."""
+    query_mask, value_mask, key_mask, attention_mask = masks
+    if return_attention_scores:
+        raise ValueError("Attention scores are not returned with rules on the scores (`attn_logits_soft_cap`, `distance_slopes`, `segment_ids`, `prefix_lengths`) or a `cache`.")
+    if dropout > 0.0:
+        raise ValueError("Dropout is not supported with `segment_ids`, `prefix_lengths` or a `cache`. Please set dropout to 0.0.")
+    if len(q.shape) != 4:
+        raise ValueError(f"Rules on the scores and a `cache` need inputs of shape (batch, time, features). Received: projected query of shape {tuple(q.shape)}")
+    if sharded and layer._distance_slopes is not None:
+        raise ValueError("`distance_slopes` are not supported where the heads are sharded.")
+    rules = dict(scale=scale, flash_attention=False if layer._flash_attention is False else None, attn_logits_soft_cap=layer._attn_logits_soft_cap, distance_slopes=_slopes_of(layer, q),
+                 sliding_window=layer._sliding_window)
+    if cache is not None:
+        if any(m is not None for m in masks) or segment_ids is not None or prefix_lengths is not None:
+            raise ValueError("A `cache` takes no masks, `segment_ids` or `prefix_lengths`.")
+        return ops.dot_product_attention(q, k, v, cache=cache, **rules)
+    mask = None
+    if query_mask is not None:
+        mask = ops.expand_dims(ops.expand_dims(ops.cast(query_mask, "bool"), 1), -1)
+    for m in (value_mask, key_mask):
+        if m is not None:
+            m = ops.expand_dims(ops.expand_dims(ops.cast(m, "bool"), 1), 1)
+            mask = m if mask is None else ops.logical_and(mask, m)
+    if attention_mask is not None:
+        m = ops.cast(attention_mask, "bool")
+        for _ in range(4 - len(m.shape)):
+            m = ops.expand_dims(m, axis=-3)
+        mask = m if mask is None else ops.logical_and(mask, m)
+    return ops.dot_product_attention(q, k, v, mask=mask, is_causal=bool(use_causal_mask), segment_ids=segment_ids, prefix_lengths=prefix_lengths, **rules)
+
+
 @keras_export("keras.layers.MultiHeadAttention")
 class MultiHeadAttention(Layer):
+    """``attn_logits_soft_cap`` and ``distance_slopes`` (one number a head), and in a call ``segment_ids``, ``prefix_lengths`` and ``cache``, are those of
+    ``ops.dot_product_attention``; a call with a ``cache`` is causal whatever ``use_causal_mask`` says and carries no gradient.
+
+    The pools of a ``cache`` are of the layer's compute type.  A model that hands caches on to its layers is of that type too: a call converts its
+    arguments, and what the layers would then write to is a copy."""
+
     def __init__(self, num_heads, key_dim, value_dim=None, dropout=0.0, use_bias=True, output_shape=None, attention_axes=None, sliding_window=None,
                  flash_attention=None, kernel_initializer="glorot_uniform", bias_initializer="zeros", kernel_regularizer=None, bias_regularizer=None,
-                 activity_regularizer=None, kernel_constraint=None, bias_constraint=None, use_gate=False, seed=None, **kwargs):
+                 activity_regularizer=None, kernel_constraint=None, bias_constraint=None, use_gate=False, seed=None, attn_logits_soft_cap=None,
+                 distance_slopes=None, **kwargs):
         for nm, v in (("num_heads", num_heads), ("key_dim", key_dim)):
             if not isinstance(v, int) or v <= 0:
                 raise ValueError(f"Received an invalid value for argument `{nm}`, expected a positive integer. Received: {nm}={v}")
@@ -100,9 +171,14 @@ class MultiHeadAttention(Layer):
             raise ValueError(f"`sliding_window` must be `None` or a positive integer. Received: sliding_window={sliding_window}")
         self._sliding_window = sliding_window
         self.seed = seed
+        _fixed_rules(self, attn_logits_soft_cap, distance_slopes, num_heads, dropout)
         self._inverse_sqrt_key_dim = 1.0 / math.sqrt(float(key_dim))
         if self._flash_attention and self._dropout > 0.0:
             raise ValueError("Dropout is not supported when flash attention is enabled. Please set dropout to 0.0 to use flash attention.")
+
+    def _convert_structure(self, x):
+        # a cache is written to: the pools themselves go on, whatever their type
+        return x if isinstance(x, dict) else super()._convert_structure(x)
 
     num_heads = property(lambda self: self._num_heads)
     key_dim = property(lambda self: self._key_dim)
@@ -130,6 +206,7 @@ class MultiHeadAttention(Layer):
             "kernel_constraint": constraints.serialize(self._kernel_constraint),
             "bias_constraint": constraints.serialize(self._bias_constraint),
             "seed": self.seed,
+            **_rules_config(self),
         }
 
     def _sublayer_kwargs(self):
@@ -212,7 +289,7 @@ class MultiHeadAttention(Layer):
         return ops.einsum(self._combine_equation, dropped, value), scores
 
     def call(self, query, value, key=None, query_mask=None, value_mask=None, key_mask=None, attention_mask=None, return_attention_scores=False,
-             training=None, use_causal_mask=False):
+             training=None, use_causal_mask=False, segment_ids=None, prefix_lengths=None, cache=None):
         if key is None:
             key = value
         # The masks are handled here, at the level of the layer: the projections below see plain tensors
@@ -224,6 +301,9 @@ class MultiHeadAttention(Layer):
         for t, _ in carried:
             t._keras_mask = None
         try:
+            if segment_ids is not None or prefix_lengths is not None or cache is not None or self._attn_logits_soft_cap is not None or self._distance_slopes is not None:
+                return self._attend_ruled(query, value, key, query_mask, value_mask, key_mask, attention_mask, return_attention_scores, use_causal_mask,
+                                          segment_ids, prefix_lengths, cache)
             return self._attend(query, value, key, query_mask, value_mask, key_mask, attention_mask, return_attention_scores, training, use_causal_mask)
         finally:
             for t, m in carried:
@@ -239,20 +319,7 @@ class MultiHeadAttention(Layer):
         else:
             attention_mask = self._compute_attention_mask(query, value, query_mask=query_mask, value_mask=value_mask, key_mask=key_mask,
                                                           attention_mask=attention_mask, use_causal_mask=use_causal_mask)
-        tp = None
-        if getattr(self._query_dense._kernel, "_shard_slices", None) is not None:
-            from keras_b200.parallel import tensor_parallel
-
-            projections = [self._query_dense, self._key_dense, self._value_dense] + ([self._gate_dense] if self._use_gate else [])
-            tp = tensor_parallel.mark_attention(self, projections, self._output_dense)
-        gate = self._gate_dense(query) if self._use_gate else None
-        joint = _joint_projections(self, query) if query is value and query is key and tp is None else None
-        if joint is not None:
-            q, k, v = joint
-        else:
-            q = self._query_dense(query)
-            k = self._key_dense(key)
-            v = self._value_dense(value)
+        q, k, v, gate, tp = self._project(query, value, key)
         out = scores = None
         if padding_only:
             out = self._attend_padded(q, k, v, query_mask, value_mask, key_mask)
@@ -271,9 +338,41 @@ class MultiHeadAttention(Layer):
                 pass
         if return_attention_scores:
             if tp is not None and scores is not None:
+                from keras_b200.parallel import tensor_parallel
+
                 scores = tensor_parallel.gather_dim(scores, 1, *tp[1:])
             return out, scores
         return out
+
+    def _attend_ruled(self, query, value, key, query_mask, value_mask, key_mask, attention_mask, return_attention_scores, use_causal_mask, segment_ids,
+                      prefix_lengths, cache):
+        if tuple(self._attention_axes) != (1,):
+            raise ValueError(f"Rules on the scores and a `cache` need attention over the first axis alone. Received: attention_axes={self._attention_axes}")
+        q, k, v, gate, tp = self._project(query, value, key)
+        out = _attend_by_rules(self, q, k, v, self._inverse_sqrt_key_dim, (query_mask, value_mask, key_mask, attention_mask), use_causal_mask, return_attention_scores,
+                               self._dropout, segment_ids, prefix_lengths, cache, tp is not None)
+        if gate is not None:
+            out = ops.multiply(out, gate)
+        out = self._output_dense(out)
+        if query_mask is not None:
+            try:
+                out._keras_mask = query_mask
+            except AttributeError:
+                pass
+        return out
+
+    def _project(self, query, value, key):
+        """Projected query, key and value, the gate or ``None``, and the marks of a layer whose heads are sharded or ``None``."""
+        tp = None
+        if getattr(self._query_dense._kernel, "_shard_slices", None) is not None:
+            from keras_b200.parallel import tensor_parallel
+
+            projections = [self._query_dense, self._key_dense, self._value_dense] + ([self._gate_dense] if self._use_gate else [])
+            tp = tensor_parallel.mark_attention(self, projections, self._output_dense)
+        gate = self._gate_dense(query) if self._use_gate else None
+        joint = _joint_projections(self, query) if query is value and query is key and tp is None else None
+        q, k, v = joint if joint is not None else (self._query_dense(query), self._key_dense(key), self._value_dense(value))
+        return q, k, v, gate, tp
 
     def _takes_padding(self):
         """Whether masks of whole rows and keys may go to the fused kernel as they are: no subclass looks at their product."""
@@ -339,7 +438,7 @@ class MultiHeadAttention(Layer):
         return query_shape
 
     def compute_output_spec(self, query, value, key=None, query_mask=None, value_mask=None, key_mask=None, attention_mask=None,
-                            return_attention_scores=False, training=None, use_causal_mask=False):
+                            return_attention_scores=False, training=None, use_causal_mask=False, segment_ids=None, prefix_lengths=None, cache=None):
         from keras_b200.core.keras_tensor import KerasTensor
 
         key_shape = key.shape if key is not None else None
@@ -355,11 +454,16 @@ class MultiHeadAttention(Layer):
 @keras_export(["keras.layers.GroupQueryAttention", "keras.layers.GroupedQueryAttention"])
 class GroupedQueryAttention(Layer):
     """Grouped-query attention (keras/src/layers/attention/grouped_query_attention.py): ``num_query_heads`` query
-    heads share ``num_key_value_heads`` key/value heads.  K/V are never repeated in memory on the fused path."""
+    heads share ``num_key_value_heads`` key/value heads.  K/V are never repeated in memory on the fused path.
+
+    ``attn_logits_soft_cap``, ``distance_slopes`` (one number a query head) and ``sliding_window``, and in a call ``segment_ids``, ``prefix_lengths`` and
+    ``cache``, are those of ``ops.dot_product_attention``; a call with a ``cache`` is causal whatever ``use_causal_mask`` says and carries no gradient
+    (``MultiHeadAttention`` says what its type has to be)."""
 
     def __init__(self, head_dim, num_query_heads, num_key_value_heads, dropout=0.0, use_bias=True, flash_attention=None,
                  kernel_initializer="glorot_uniform", bias_initializer="zeros", kernel_regularizer=None, bias_regularizer=None,
-                 activity_regularizer=None, kernel_constraint=None, bias_constraint=None, use_gate=False, seed=None, **kwargs):
+                 activity_regularizer=None, kernel_constraint=None, bias_constraint=None, use_gate=False, seed=None, attn_logits_soft_cap=None,
+                 distance_slopes=None, sliding_window=None, **kwargs):
         super().__init__(**kwargs)
         self.supports_masking = True
         self.head_dim, self.num_query_heads, self.num_key_value_heads = head_dim, num_query_heads, num_key_value_heads
@@ -376,10 +480,18 @@ class GroupedQueryAttention(Layer):
         self.kernel_constraint = constraints.get(kernel_constraint)
         self.bias_constraint = constraints.get(bias_constraint)
         self.seed = seed
+        _fixed_rules(self, attn_logits_soft_cap, distance_slopes, num_query_heads, dropout)
+        self._sliding_window = None if sliding_window is None else attention_rules.window(sliding_window)
+        if dropout > 0.0 and sliding_window is not None:
+            raise ValueError("Dropout is not supported with `sliding_window`. Please set dropout to 0.0.")
         self._inverse_sqrt_head_dim = 1.0 / math.sqrt(float(head_dim))
         self._return_attention_scores = False
         if self._flash_attention and self.dropout > 0.0:
             raise ValueError("Dropout is not supported when flash attention is enabled. Please set dropout to 0.0 to use flash attention.")
+
+    def _convert_structure(self, x):
+        # a cache is written to: the pools themselves go on, whatever their type
+        return x if isinstance(x, dict) else super()._convert_structure(x)
 
     def _kw(self):
         return dict(kernel_initializer=self.kernel_initializer.__class__.from_config(self.kernel_initializer.get_config()),
@@ -418,16 +530,39 @@ class GroupedQueryAttention(Layer):
     output_dense = property(lambda self: self._output_dense)
 
     def call(self, query, value, key=None, query_mask=None, value_mask=None, key_mask=None, attention_mask=None, return_attention_scores=False,
-             training=None, use_causal_mask=False):
+             training=None, use_causal_mask=False, segment_ids=None, prefix_lengths=None, cache=None):
         self._return_attention_scores = return_attention_scores
         if key is None:
             key = value
+        if any(a is not None for a in (segment_ids, prefix_lengths, cache, self._attn_logits_soft_cap, self._distance_slopes, self._sliding_window)):
+            q, k, v, gate, tp = self._project(query, value, key)
+            out = _attend_by_rules(self, q, k, v, self._inverse_sqrt_head_dim, (query_mask, value_mask, key_mask, attention_mask), use_causal_mask,
+                                   return_attention_scores, self.dropout, segment_ids, prefix_lengths, cache, tp is not None)
+            return self._output_dense(out if gate is None else ops.multiply(out, gate))
         # a purely causal mask is passed to the fused attention kernel as a flag instead of a [T, T] tensor
         self._causal_only = bool(use_causal_mask and query_mask is None and value_mask is None and key_mask is None and attention_mask is None
                                  and self.dropout == 0.0 and not return_attention_scores and self._flash_attention is not False)
         if not self._causal_only:
             attention_mask = self._compute_attention_mask(query, value, query_mask=query_mask, value_mask=value_mask, key_mask=key_mask,
                                                           attention_mask=attention_mask, use_causal_mask=use_causal_mask)
+        q, k, v, gate, tp = self._project(query, value, key)
+        out, scores = self._compute_attention(q, k, v, attention_mask=attention_mask, training=training)
+        if gate is not None:
+            out = ops.multiply(out, gate)
+        out = self._output_dense(out)
+        if return_attention_scores:
+            if tp is not None and scores is not None:
+                from keras_b200.parallel import tensor_parallel
+
+                scores = tensor_parallel.gather_dim(scores, 1, *tp[1:])
+            return out, scores
+        return out
+
+    _compute_attention_mask = MultiHeadAttention._compute_attention_mask
+    _compute_causal_mask = MultiHeadAttention._compute_causal_mask
+
+    def _project(self, query, value, key):
+        """Projected query, key and value, the gate or ``None``, and the marks of a layer whose heads are sharded or ``None``."""
         tp = None
         if getattr(self._query_dense._kernel, "_shard_slices", None) is not None:
             from keras_b200.parallel import tensor_parallel
@@ -436,25 +571,8 @@ class GroupedQueryAttention(Layer):
             tp = tensor_parallel.mark_attention(self, projections, self._output_dense)
         gate = self._gate_dense(query) if self.use_gate else None
         joint = _joint_projections(self, query) if query is value and query is key and tp is None else None
-        if joint is not None:
-            q, k, v = joint
-        else:
-            q = self._query_dense(query)
-            k = self._key_dense(key)
-            v = self._value_dense(value)
-        out, scores = self._compute_attention(q, k, v, attention_mask=attention_mask, training=training)
-        if gate is not None:
-            out = ops.multiply(out, gate)
-        out = self._output_dense(out)
-        if return_attention_scores:
-            if tp is not None and scores is not None:
-                scores = tensor_parallel.gather_dim(scores, 1, *tp[1:])
-            return out, scores
-        return out
-
-    _compute_attention_mask = MultiHeadAttention._compute_attention_mask
-    _compute_causal_mask = MultiHeadAttention._compute_causal_mask
-    _sliding_window = None
+        q, k, v = joint if joint is not None else (self._query_dense(query), self._key_dense(key), self._value_dense(value))
+        return q, k, v, gate, tp
 
     def _masked_softmax(self, scores, attention_mask=None):
         if attention_mask is not None:
@@ -501,6 +619,8 @@ class GroupedQueryAttention(Layer):
             "activity_regularizer": regularizers.serialize(self.activity_regularizer),
             "kernel_constraint": constraints.serialize(self.kernel_constraint), "bias_constraint": constraints.serialize(self.bias_constraint),
             "seed": self.seed,
+            **_rules_config(self),
+            **({} if self._sliding_window is None else {"sliding_window": self._sliding_window}),
         }
 
 

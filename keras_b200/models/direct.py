@@ -347,8 +347,10 @@ def _attention(layer, x, causal, mask=None):
     grouped = type(layer) is GroupedQueryAttention
     if x is None or x.ndim != 3 or not _ordinary(layer) or d["_input_spec"] is not None or d["_flash_attention"] is False:
         return None
+    if d["_attn_logits_soft_cap"] is not None or d["_distance_slopes"] is not None:
+        return None
     if grouped:
-        if d["dropout"] != 0.0 or d["use_gate"]:
+        if d["dropout"] != 0.0 or d["use_gate"] or d["_sliding_window"] is not None:
             return None
         heads, kv, size, scale = d["num_query_heads"], d["num_key_value_heads"], d["head_dim"], d["_inverse_sqrt_head_dim"]
     else:

@@ -15,6 +15,7 @@ from keras_b200.core import config
 from keras_b200.core.dtypes import result_type, standardize_dtype, to_torch_dtype
 from keras_b200.core.tensor import convert_to_tensor
 from keras_b200.kernels import dispatch
+from keras_b200.ops import attention_rules
 from keras_b200.ops._dispatch import op
 from keras_b200.ops.numpy import _floatize, _t
 
@@ -687,8 +688,35 @@ def _whole_rows(t, T, S):
 
 
 @op("nn")
-def dot_product_attention(query, key, value, bias=None, mask=None, scale=None, is_causal=False, flash_attention=None, attn_logits_soft_cap=None):
-    """Inputs are ``[B, T, N, H]`` / ``[B, S, K, H]`` (K divides N: grouped-query)."""
+def dot_product_attention(query, key, value, bias=None, mask=None, scale=None, is_causal=False, flash_attention=None, attn_logits_soft_cap=None,
+                          distance_slopes=None, sliding_window=None, segment_ids=None, prefix_lengths=None, cache=None):
+    """Inputs are ``[B, T, N, H]`` / ``[B, S, K, H]`` (K divides N: grouped-query).
+
+    ``attn_logits_soft_cap``: scores become ``cap * tanh(score / cap)``.
+
+    Rules about who sees whom, and a bias by distance, take the place of ``[T, S]`` masks and biases and can be combined with each other, with the cap
+    and with ``is_causal``.  Both directions run on this package's kernels for float32, bfloat16 and float16 heads of up to 256; together with
+    ``bias`` or ``mask`` they run in elementary operations.
+
+    * ``distance_slopes``: one number a query head, ``[N]``; ``slope * |i - j|`` is taken from the score of row i and key j.  Constants; to be recorded
+      into a CUDA graph they have to be a tensor on the device.
+    * ``sliding_window``: row i sees the keys with ``|i - j| < sliding_window``.
+    * ``segment_ids``: int32 ``[B, T]``, or a tuple of those of the rows ``[B, T]`` and of the keys ``[B, S]``.  Rows see the keys of their own segment; a negative
+      id is padding, which sees nothing and is seen by nobody.  Ids may come in any order; tiles without a common id are left out.
+    * ``prefix_lengths``: int32 ``[B]``, with ``is_causal``: the first keys of each sequence, as many as that, are seen by every row.
+
+    With any of the four, a row that sees nothing is zero and has no gradient (a fully masked row of ``mask`` alone attends uniformly).  Values
+    that nobody may see have to be finite all the same: they are multiplied with zero.
+
+    ``cache``: attention of new tokens over a paged key/value cache.  A dict of ``key`` and ``value``, pools ``[pages, positions, K, H]`` of the inputs' type;
+    ``pages``, int32 ``[B, n]``, the pool's page for the positions ``i * positions`` .. of each sequence; and ``lengths``, int32 ``[B]``, the positions that are
+    taken already.  Query, key and value are those of ``T`` new tokens a sequence.  Their keys and values are written to the pools, at
+    ``lengths`` .. ``lengths + T - 1``, and token t sees the positions up to ``lengths + t``.  The caller advances ``lengths`` once all layers have run.
+    A negative length marks an idle sequence: nothing is written and its rows are zero.  A position without a page (behind the table's
+    end, or a number that is no page) is neither read nor written: its rows are NaN on a GPU, and an error on the CPU.  Positions behind a
+    sequence's end may hold anything.  Two sequences may share pages that neither writes to.  No gradients; ``bias``, ``mask``, ``segment_ids`` and
+    ``prefix_lengths`` are refused.
+    """
     q, k, v = _t(query), _t(key), _t(value)
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
         raise ValueError(f"`dot_product_attention` only supports 4D inputs. Received: query.shape={tuple(q.shape)}, key.shape={tuple(k.shape)}, value.shape={tuple(v.shape)}.")
@@ -696,6 +724,19 @@ def dot_product_attention(query, key, value, bias=None, mask=None, scale=None, i
     q, k, v = q.to(d), k.to(d), v.to(d)
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
+    if cache is not None:
+        if any(a is not None for a in (bias, mask, segment_ids, prefix_lengths)):
+            raise ValueError("`dot_product_attention`: a cache takes no `bias`, `mask`, `segment_ids` or `prefix_lengths`.")
+        return attention_rules.attend_cached(q, k, v, cache, scale, attn_logits_soft_cap, distance_slopes, sliding_window, flash_attention is not False)
+    if any(a is not None for a in (distance_slopes, sliding_window, segment_ids, prefix_lengths)):
+        if flash_attention and bias is not None:
+            raise ValueError("Flash attention does not support `bias`.")
+        rules = attention_rules.make(q, k, v, scale, is_causal, attn_logits_soft_cap, distance_slopes, sliding_window, segment_ids, prefix_lengths)
+        return attention_rules.attend(q, k, v, rules, None if bias is None else _t(bias), None if mask is None else _t(mask), flash_attention is not False)
+    if attn_logits_soft_cap is not None and bias is None and mask is None and flash_attention is None:
+        capped = attention_rules.capped(q, k, v, scale, is_causal, attn_logits_soft_cap)
+        if capped is not None:
+            return capped
     if bias is None and attn_logits_soft_cap is None and flash_attention is not False:
         fused = dispatch.flash_attention(q, k, v, _t(mask) if mask is not None else None, scale, is_causal)
         if fused is not None:
