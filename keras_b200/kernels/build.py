@@ -26,7 +26,8 @@ NVCC_FLAGS = [
 ]
 
 # Sources whose float32 results stand next to the library's own float32 math: exact division and full-accuracy functions.
-PRECISE = {"lstm.cu", "sgemm.cu", "xent_classes.cu", "metrics.cu", "attention_rules.cu", "attention_cache.cu"}
+PRECISE = {"lstm.cu", "sgemm.cu", "xent_classes.cu", "metrics.cu", "attention_rules.cu", "attention_cache.cu", "attention_rules_fwd_sm100.cu",
+           "attention_rules_bwd_sm100.cu"}
 
 
 def _flags(src):

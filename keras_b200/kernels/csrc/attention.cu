@@ -29,10 +29,11 @@
 //
 // Every mbarrier wait is bounded (iteration limit + abort flag): on expiry the kernel writes a code to *err, lets its
 // outstanding copies land, frees TMEM and returns.
-#include "gemm_sm100.cuh"
+#include "attention_sm100.cuh"
 
 namespace {
 using namespace kbgemm;
+using namespace kbattn;
 
 struct FlashParams {
   int B, H, Hkv, Tq, Tk;
@@ -46,17 +47,6 @@ struct FlashParams {
   long long row_mask_b;
 };
 
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
-  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-               ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-               : "memory");
-}
-__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2, int c3) {
-  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
-               ::"l"(map), "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-               : "memory");
-}
-
 template <int D, int NT>
 struct FlashCfg {
   static constexpr int CH = D / 64;                   // 64-column chunks of the head dimension
@@ -68,74 +58,6 @@ struct FlashCfg {
   static constexpr int THREADS_ = NT == 2 ? 384 : 192;
 };
 
-__device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
-// 2^x of two values on the FMA pipe, for the share of the exponentials that the special-function pipe has no time for.
-// x = n + f with n the nearest integer (the sum with 1.5 * 2^23 leaves n in the low bits), 2^f on [-1/2, 1/2] by a polynomial of
-// degree 5 with the least maximum relative error (a linear program over 4000 Chebyshev points gives its coefficients, rounded to float32;
-// 2.1e-7 in float32, as the hardware's own approximation), n added to the exponent.  x is at
-// most RESCALE_LOG2; below -126 the result is held at 2^-126, which is nothing beside a row sum of at least 2^-8.
-__device__ __forceinline__ void exp2_poly2(uint64_t x2, float& y0, float& y1) {
-  float x0, x1;
-  unpack_f32x2(x2, x0, x1);
-  const uint64_t x = pack_f32x2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
-  const uint64_t t = add_f32x2(x, pack_f32x2(12582912.f, 12582912.f));  // n in the low bits
-  const uint64_t n = add_f32x2(t, pack_f32x2(-12582912.f, -12582912.f));
-  const uint64_t f = fma_f32x2(n, pack_f32x2(-1.f, -1.f), x);
-  uint64_t y = fma_f32x2(pack_f32x2(0.001327647129073739f, 0.001327647129073739f), f, pack_f32x2(0.009675540961325169f, 0.009675540961325169f));
-  y = fma_f32x2(y, f, pack_f32x2(0.05550713092088699f, 0.05550713092088699f));
-  y = fma_f32x2(y, f, pack_f32x2(0.24022120237350464f, 0.24022120237350464f));
-  y = fma_f32x2(y, f, pack_f32x2(0.6931469440460205f, 0.6931469440460205f));
-  y = fma_f32x2(y, f, pack_f32x2(1.0000001192092896f, 1.0000001192092896f));
-  float t0, t1;
-  unpack_f32x2(t, t0, t1);
-  unpack_f32x2(y, y0, y1);
-  y0 = __uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23));
-  y1 = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23));
-}
 constexpr int POLY_EVERY = 4;           // one pair of exponentials in four
 
 constexpr float MASKED = -1e30f;        // of a score, before scaling: finite, so that a row of nothing else is uniform
@@ -508,20 +430,6 @@ int launch_flash_any(const CUtensorMap& q, const CUtensorMap& k, const CUtensorM
   if (p.Tq <= 128)  // a single tile of rows: two such CTAs share an SM
     return p.mask ? launch_flash<D, 1, true>(q, k, v, o, p, stream) : launch_flash<D, 1, false>(q, k, v, o, p, stream);
   return p.mask ? launch_flash<D, 2, true>(q, k, v, o, p, stream) : launch_flash<D, 2, false>(q, k, v, o, p, stream);
-}
-
-// 4-D bf16 tensor map over [batch, time, heads, head_dim] storage: dims (head_dim, time, heads, batch).
-bool make_map_bthd(CUtensorMap* map, const void* ptr, int D, int T, int H, int B, long long stride_t, long long stride_h, long long stride_b, int box_d,
-                   int box_t) {
-  EncodeTiledFn fn = get_encode_fn();
-  if (fn == nullptr) return false;
-  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)H, (cuuint64_t)B};
-  cuuint64_t strides[3] = {(cuuint64_t)stride_t * 2, (cuuint64_t)stride_h * 2, (cuuint64_t)stride_b * 2};
-  cuuint32_t box[4] = {(cuuint32_t)box_d, (cuuint32_t)box_t, 1, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS;
 }
 
 }  // namespace

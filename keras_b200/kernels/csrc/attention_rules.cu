@@ -119,11 +119,12 @@ __device__ __forceinline__ float rule_score(const Rules& r, const Score& f, floa
 struct Gradients {
   const void* grad_out;
   Strides go;
-  const float *lse, *delta;
+  const float *lse, *delta;  // [B, H, pitch]
+  int pitch;
 };
 
 template <typename T, int DP, int BT>
-__global__ void __launch_bounds__(256) rules_fwd_kernel(const Rules r, const T* q, Strides qs, const T* k, Strides ks, const T* v, Strides vs, T* o, float* lse, int vec) {
+__global__ void __launch_bounds__(256) rules_fwd_kernel(const Rules r, const T* q, Strides qs, const T* k, Strides ks, const T* v, Strides vs, T* o, float* lse, int pitch, int vec) {
   using C = Tile<T, DP, BT>;
   constexpr int M = BT / 16;
   extern __shared__ __align__(16) float sm[];
@@ -200,24 +201,39 @@ __global__ void __launch_bounds__(256) rules_fwd_kernel(const Rules r, const T* 
   for (int i = 0; i < M; ++i) {
     inv[i] = l[i] == 0.f ? 0.f : 1.f / l[i];
     const int t = q0 + ty + 16 * i;
-    if (lse != nullptr && tx == 0 && t < r.Tq) lse[((long long)b * r.H + h) * r.Tq + t] = l[i] == 0.f ? INFINITY : m[i] + log2f(l[i]);
+    if (lse != nullptr && tx == 0 && t < r.Tq) lse[((long long)b * r.H + h) * pitch + t] = l[i] == 0.f ? INFINITY : m[i] + log2f(l[i]);
   }
   store_rows<T, DP, M>(o + ((long long)b * r.Tq * r.H + h) * r.D, (long long)r.H * r.D, acc, inv, q0, r.Tq, r.D, ty, tx);
 }
 
-// delta[b, h, t] = sum_d grad_out * o, a warp a row; o is contiguous.
+// delta[b, h, t] = sum_d grad_out * (o + lo), a warp a row; o and lo (null: none) are contiguous.  Rows between Tq and `pitch` get zeros.
+// 16-bit heads whose lanes have 16 bytes each are read as vectors.
 template <typename T>
-__global__ void __launch_bounds__(256) rules_delta_kernel(const T* o, const T* go, Strides gs, float* delta, int B, int H, int Tq, int D) {
+__global__ void __launch_bounds__(256) rules_delta_kernel(const T* o, const T* lo, const T* go, Strides gs, float* delta, int B, int H, int Tq, int pitch, int D, int vec) {
   const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= (long long)B * Tq * H) return;
-  const int h = (int)(row % H);
+  if (row >= (long long)B * pitch * H) return;
+  const int h = (int)(row % H), lane = threadIdx.x & 31;
   const long long bt = row / H;
-  const int t = (int)(bt % Tq), b = (int)(bt / Tq);
-  const T *x = o + row * D, *y = go + b * gs.b + t * gs.t + h * gs.h;
+  const int t = (int)(bt % pitch), b = (int)(bt / pitch);
   float sum = 0.f;
-  for (int d = threadIdx.x & 31; d < D; d += 32) sum = fmaf(load_f32(x + d), load_f32(y + d), sum);
-  sum = warp_sum(sum);
-  if ((threadIdx.x & 31) == 0) delta[((long long)b * H + h) * Tq + t] = sum;
+  if (t < Tq) {
+    const long long at = (((long long)b * Tq + t) * H + h) * D;
+    const T *x = o + at, *z = lo + at, *y = go + b * gs.b + t * gs.t + h * gs.h;
+    if (vec) {
+      constexpr int V = 16 / sizeof(T);
+      for (int d = lane * V; d < D; d += 32 * V) {
+        const uint4 a = *reinterpret_cast<const uint4*>(x + d), c = *reinterpret_cast<const uint4*>(y + d);
+        const uint4 e = lo != nullptr ? *reinterpret_cast<const uint4*>(z + d) : make_uint4(0, 0, 0, 0);
+        const T *xa = reinterpret_cast<const T*>(&a), *yc = reinterpret_cast<const T*>(&c), *ze = reinterpret_cast<const T*>(&e);
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum = fmaf(to_f32<T>(xa[i]) + (lo != nullptr ? to_f32<T>(ze[i]) : 0.f), to_f32<T>(yc[i]), sum);
+      }
+    } else {
+      for (int d = lane; d < D; d += 32) sum = fmaf(load_f32(x + d) + (lo != nullptr ? load_f32(z + d) : 0.f), load_f32(y + d), sum);
+    }
+    sum = warp_sum(sum);
+  }
+  if (lane == 0) delta[((long long)b * H + h) * pitch + t] = sum;
 }
 
 // Probability of a pair and the gradient of its plain score, from the sums that the forward pass kept.
@@ -254,7 +270,7 @@ __global__ void __launch_bounds__(256) rules_dkv_kernel(const Rules r, const T* 
   rows_of_keys(r, k0, min(k0 + BT, r.Tk) - 1, prefix, first, last);
   for (int h = hkv * group; h < (hkv + 1) * group; ++h) {
     const Score f = score_of(r, h);
-    const float *lse = g.lse + ((long long)b * r.H + h) * r.Tq, *delta = g.delta + ((long long)b * r.H + h) * r.Tq;
+    const float *lse = g.lse + ((long long)b * r.H + h) * g.pitch, *delta = g.delta + ((long long)b * r.H + h) * g.pitch;
     for (int q0 = first / BT * BT; q0 <= last; q0 += BT) {
       if (!segments_meet(r, b, q0, k0)) continue;
       __syncthreads();
@@ -322,7 +338,7 @@ __global__ void __launch_bounds__(256) rules_dq_kernel(const Rules r, const T* q
 #pragma unroll
   for (int i = 0; i < M; ++i) {
     const int t = q0 + ty + 16 * i;
-    const long long at = ((long long)b * r.H + h) * r.Tq + t;
+    const long long at = ((long long)b * r.H + h) * g.pitch + t;
     row_span(r, t, prefix, lo[i], hi[i]);
     seg[i] = r.seg_q != nullptr && t < r.Tq ? r.seg_q[(long long)b * r.Tq + t] : 0;
     if (t >= r.Tq || seg[i] < 0) hi[i] = -1;
@@ -391,7 +407,7 @@ bool vectors(const void* p, const Strides& s, int D) {
 }
 
 template <typename T, int DP, int BT>
-int rules_fwd(const Rules& r, const void* q, Strides qs, const void* k, Strides ks, const void* v, Strides vs, void* o, float* lse, cudaStream_t stream) {
+int rules_fwd(const Rules& r, const void* q, Strides qs, const void* k, Strides ks, const void* v, Strides vs, void* o, float* lse, int pitch, cudaStream_t stream) {
   using C = Tile<T, DP, BT>;
   constexpr int SMEM = (3 * C::FLOATS + BT * C::SP) * 4;
   static bool attr[KB_MAX_DEVICES] = {false};
@@ -400,7 +416,7 @@ int rules_fwd(const Rules& r, const void* q, Strides qs, const void* k, Strides 
     return -3;
   }
   const int vec = (vectors<T>(q, qs, r.D) ? 1 : 0) | (vectors<T>(k, ks, r.D) ? 2 : 0) | (vectors<T>(v, vs, r.D) ? 4 : 0);
-  rules_fwd_kernel<T, DP, BT><<<(unsigned)((long long)((r.Tq + BT - 1) / BT) * r.H * r.B), 256, SMEM, stream>>>(r, (const T*)q, qs, (const T*)k, ks, (const T*)v, vs, (T*)o, lse, vec);
+  rules_fwd_kernel<T, DP, BT><<<(unsigned)((long long)((r.Tq + BT - 1) / BT) * r.H * r.B), 256, SMEM, stream>>>(r, (const T*)q, qs, (const T*)k, ks, (const T*)v, vs, (T*)o, lse, pitch, vec);
   return 0;
 }
 template <typename T, int DP, int BT>
@@ -464,16 +480,16 @@ bool check(const Rules& r, int dtype) {
     }                                                                 \
   } while (0)
 
-// q [B, Tq, H, D], k and v [B, Tk, Hkv, D] with unit stride on D; o [B, Tq, H, D] contiguous; lse [B, H, Tq] (log2 units; +inf: a row that sees
-// nothing) may be null.  dtype 0 float32, 1 bfloat16, 2 float16.
-KB_API int kb200_attention_rules_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const long long* strides, int dtype, int B, int H, int Hkv, int Tq, int Tk,
-                                     int D, float scale, float cap, const float* slopes, int causal, int window, const int* prefix, const int* seg_q, const int* seg_k,
+// q [B, Tq, H, D], k and v [B, Tk, Hkv, D] with unit stride on D; o [B, Tq, H, D] contiguous; lse [B, H, pitch] (log2 units; +inf: a row that
+// sees nothing) may be null.  dtype 0 float32, 1 bfloat16, 2 float16.
+KB_API int kb200_attention_rules_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int pitch, const long long* strides, int dtype, int B, int H, int Hkv, int Tq,
+                                     int Tk, int D, float scale, float cap, const float* slopes, int causal, int window, const int* prefix, const int* seg_q, const int* seg_k,
                                      const void* range_q, const void* range_k, cudaStream_t stream) {
   const Rules r{B, H, Hkv, Tq, Tk, D, scale, cap, slopes, causal, window, prefix, seg_q, seg_k, (const int4*)range_q, (const int4*)range_k};
   if (!check(r, dtype)) return -2;
   const Strides qs{strides[0], strides[1], strides[2]}, ks{strides[3], strides[4], strides[5]}, vs{strides[6], strides[7], strides[8]};
   int rc = 0;
-#define KB_CALL(T, DP, BT) rules_fwd<T, DP, BT>(r, q, qs, k, ks, v, vs, o, lse, stream)
+#define KB_CALL(T, DP, BT) rules_fwd<T, DP, BT>(r, q, qs, k, ks, v, vs, o, lse, pitch, stream)
   KB_RULES_DISPATCH(KB_CALL);
 #undef KB_CALL
   if (rc != 0) return rc;
@@ -481,25 +497,36 @@ KB_API int kb200_attention_rules_fwd(const void* q, const void* k, const void* v
   return 0;
 }
 
-// delta [B, H, Tq]: for each row the sum of grad_out * o.
-KB_API int kb200_attention_rules_delta(const void* o, const void* grad_out, const long long* strides, float* delta, int dtype, int B, int H, int Tq, int D, cudaStream_t stream) {
+// delta [B, H, pitch]: for each row the sum of grad_out * (o + lo); lo may be null.
+KB_API int kb200_attention_rules_delta(const void* o, const void* lo, const void* grad_out, const long long* strides, float* delta, int pitch, int dtype, int B, int H, int Tq, int D,
+                                       cudaStream_t stream) {
   const Strides gs{strides[0], strides[1], strides[2]};
-  const unsigned grid = (unsigned)(((long long)B * Tq * H + 7) / 8);
-  if (dtype == 0) rules_delta_kernel<float><<<grid, 256, 0, stream>>>((const float*)o, (const float*)grad_out, gs, delta, B, H, Tq, D);
-  else if (dtype == 1) rules_delta_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>((const __nv_bfloat16*)o, (const __nv_bfloat16*)grad_out, gs, delta, B, H, Tq, D);
-  else rules_delta_kernel<__half><<<grid, 256, 0, stream>>>((const __half*)o, (const __half*)grad_out, gs, delta, B, H, Tq, D);
+  const long long blocks = ((long long)B * pitch * H + 7) / 8;
+  if (pitch < Tq || blocks > 0x7fffffffll || dtype < 0 || dtype > 2) {
+    kb200_set_error("attention_rules_delta: sizes out of range");
+    return -2;
+  }
+  const Strides os{(long long)H * D, D, (long long)Tq * H * D};
+  const unsigned grid = (unsigned)blocks;
+#define KB_DELTA(T)                                                                                                                                               \
+  rules_delta_kernel<T><<<grid, 256, 0, stream>>>((const T*)o, (const T*)lo, (const T*)grad_out, gs, delta, B, H, Tq, pitch, D,                                    \
+                                                  vectors<T>(o, os, D) && vectors<T>(lo, os, D) && vectors<T>(grad_out, gs, D))
+  if (dtype == 0) KB_DELTA(float);
+  else if (dtype == 1) KB_DELTA(__nv_bfloat16);
+  else KB_DELTA(__half);
+#undef KB_DELTA
   KB_CHECK_LAUNCH("attention_rules_delta");
   return 0;
 }
 
 // Gradients of the above: dq [B, Tq, H, D], dk and dv [B, Tk, Hkv, D] contiguous; dq, or dk and dv together, may be null.
-KB_API int kb200_attention_rules_bwd(const void* q, const void* k, const void* v, const void* grad_out, const long long* strides, const float* lse, const float* delta, void* dq,
-                                     void* dk, void* dv, int dtype, int B, int H, int Hkv, int Tq, int Tk, int D, float scale, float cap, const float* slopes, int causal, int window,
+KB_API int kb200_attention_rules_bwd(const void* q, const void* k, const void* v, const void* grad_out, const long long* strides, const float* lse, const float* delta, int pitch,
+                                     void* dq, void* dk, void* dv, int dtype, int B, int H, int Hkv, int Tq, int Tk, int D, float scale, float cap, const float* slopes, int causal, int window,
                                      const int* prefix, const int* seg_q, const int* seg_k, const void* range_q, const void* range_k, cudaStream_t stream) {
   const Rules r{B, H, Hkv, Tq, Tk, D, scale, cap, slopes, causal, window, prefix, seg_q, seg_k, (const int4*)range_q, (const int4*)range_k};
   if (!check(r, dtype)) return -2;
   const Strides qs{strides[0], strides[1], strides[2]}, ks{strides[3], strides[4], strides[5]}, vs{strides[6], strides[7], strides[8]};
-  const Gradients g{grad_out, {strides[9], strides[10], strides[11]}, lse, delta};
+  const Gradients g{grad_out, {strides[9], strides[10], strides[11]}, lse, delta, pitch};
   int rc = 0;
 #define KB_CALL(T, DP, BT) rules_bwd<T, DP, BT>(r, q, qs, k, ks, v, vs, g, dq, dk, dv, stream)
   KB_RULES_DISPATCH(KB_CALL);

@@ -1,0 +1,653 @@
+// Gradients of attention with scores by rule on tcgen05 tensor cores, for 16-bit heads of up to 128 (attention_rules.cuh says what a score is and
+// which keys a row sees; attention_rules.cu has the formulas).  Two kernels without atomics, so that gradients repeat bit for bit:
+//
+//   rules_dkv  a CTA a tile of 128 keys; walks over the query heads of its group and their tiles of 128 rows.
+//              S^T = K Q^T and dP^T = V dO^T in TMEM; P^T and dS^T go back to TMEM in 16 bits, as the operands of dV += P^T dO and dK += dS^T Q
+//   rules_dq   a CTA a tile of 128 rows; walks over the tiles of keys.
+//              S = Q K^T (two buffers), dP = dO V^T, dS back to TMEM as the operand of dQ += dS K
+//
+// Eight warps work on the scores: two threads a TMEM lane, each with 64 of its 128 columns, so that neither needs a shuffle.  With the lane
+// a key (dkv) or a row (dq), every operand is a tile as TMA brought it: the same tile is read along its rows for one product and across
+// them for the other.  Products run in issue order: S of the next tile may be queued behind the product that reads P from the same columns,
+// while the threads are still busy with dS.
+// What bounds them: four and three products of 128 x 128 x D a tile (D = 128: 2048 and 1536 cycles) against 64 scores a thread with an
+// exponential each, about 1000 cycles for two warps a scheduler, twice that with a cap.
+//
+// Every mbarrier wait is bounded; on expiry the kernel writes a code to *err, lets its copies land, frees TMEM and returns.
+#include "attention_rules_sm100.cuh"
+
+namespace {
+using namespace kbrules;
+
+struct Sums {
+  const float *lse, *delta;  // [B, H, pitch], pitch a multiple of 128; rows beyond Tq hold +inf and 0
+  int pitch;
+};
+
+// From 32 raw scores (columns e of a lane) to probabilities x and w = P (1 - tanh^2).  `from - e` is the distance of the pair.
+struct Lane {
+  Score f;
+  bool cap;
+  float from;
+};
+template <typename Lse>
+__device__ __forceinline__ void probabilities(float (&x)[32], float* w, const Lane& s, uint32_t keep, bool whole, Lse lse2) {
+  if (s.cap) {
+    capped(x, s.f.pre);
+    const uint64_t post2 = both(s.f.post);
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      const uint64_t t = pack_f32x2(x[e], x[e + 1]);
+      unpack_f32x2(fma_f32x2(mul_f32x2(t, both(-1.f)), t, both(1.f)), w[e], w[e + 1]);
+      unpack_f32x2(mul_f32x2(t, post2), x[e], x[e + 1]);
+    }
+  }
+  const uint64_t scale2 = both(s.cap ? 1.f : s.f.post);
+  if (s.f.slope != 0.f) {
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      unpack_f32x2(mul_f32x2(pack_f32x2(x[e], x[e + 1]), scale2), x[e], x[e + 1]);
+      x[e] = fmaf(-s.f.slope, fabsf(s.from - (float)e), x[e]);
+      x[e + 1] = fmaf(-s.f.slope, fabsf(s.from - (float)(e + 1)), x[e + 1]);
+      unpack_f32x2(add_f32x2(pack_f32x2(x[e], x[e + 1]), mul_f32x2(lse2(e), both(-1.f))), x[e], x[e + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) unpack_f32x2(fma_f32x2(pack_f32x2(x[e], x[e + 1]), scale2, mul_f32x2(lse2(e), both(-1.f))), x[e], x[e + 1]);
+  }
+  if (!whole) {
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      if (!(keep >> e & 1u)) x[e] = -INFINITY;
+  }
+#pragma unroll
+  for (int e = 0; e < 32; ++e) {
+    x[e] = ex2(x[e]);
+    w[e] = s.cap ? w[e] * x[e] : x[e];
+  }
+}
+
+// Pulls the tail of a 32-column slice of TMEM into 16-byte stores of one row.
+template <typename T>
+__device__ __forceinline__ void store_row(T* to, uint32_t tmem, int col, int D, float factor, bool valid, bool zero) {
+  float o[32];
+  if (!zero) {
+    tmem_ld32(tmem, reinterpret_cast<uint32_t*>(o));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = zero ? 0u : pack_16<T>(o[u * 8 + 2 * e] * factor, o[u * 8 + 2 * e + 1] * factor);
+    if (valid && col + u * 8 < D) *reinterpret_cast<uint4*>(to + col + u * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+constexpr int BWD_THREADS = 320;
+
+// ------------------------------------------------------------------------------------------------ dK, dV
+template <int D>
+struct DkvCfg {
+  static constexpr int CH = D / 64, TILE = CH * 16384, STAGES = D == 128 ? 2 : 4, STAGE = 2 * TILE;
+  static constexpr int BARS = 2 * TILE + STAGES * STAGE, SUMS = BARS + 256, FLAGS = SUMS + STAGES * 1024;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(BWD_THREADS, 1)
+rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                const __grid_constant__ CUtensorMap map_g, const Rules p, const Sums sums, T* dk, T* dv, int* err) {
+  using C = DkvCfg<D>;
+  constexpr int TILE = C::TILE, ST = C::STAGES;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t base = smem_u32(smem_raw);
+  if (base & 1023u) {
+    if (threadIdx.x == 0 && err) atomicExch(err, 50);
+    return;
+  }
+  const uint32_t sK = base, sV = base + TILE, sQG = base + 2 * TILE, bar_base = base + C::BARS;
+  uint8_t* flags = smem_raw + C::FLAGS;
+  const uint32_t kv_bar = bar_base, s_full = bar_base + 8, dp_full = bar_base + 16, p_ready = bar_base + 24, ds_ready = bar_base + 32, all_done = bar_base + 40;
+  auto full = [&](int s) { return bar_base + 48u + 8u * s; };
+  auto empty = [&](int s) { return bar_base + 48u + 8u * (ST + s); };
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem_raw + C::BARS + 48 + 16 * ST);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int groups = p.Hkv * p.B, k0 = (int)(blockIdx.x / groups) * BLK;  // a causal mask gives the first keys the most rows
+  const int hkv = (int)(blockIdx.x % groups) % p.Hkv, b = (int)(blockIdx.x % groups) / p.Hkv, group = p.H / p.Hkv;
+  const int prefix = p.prefix != nullptr ? p.prefix[b] : 0;
+  int first, last;  // tiles of rows
+  rows_of_keys(p, k0, min(k0 + BLK, p.Tk) - 1, prefix, first, last);
+  first /= BLK;
+  last = last < 0 ? -1 : last / BLK;
+  for (int n = threadIdx.x; first + n <= last; n += BWD_THREADS) flags[n] = (uint8_t)tile_flags(p, b, (first + n) * BLK, k0, prefix);
+  const int end = last - first + 1;
+  auto next = [&](int n) {
+    do ++n;
+    while (n < end && !(flags[n] & NEEDED));
+    return n;
+  };
+  if (threadIdx.x == 0) {
+    mbar_init(kv_bar, 1);
+    mbar_init(s_full, 1);
+    mbar_init(dp_full, 1);
+    mbar_init(p_ready, 8);
+    mbar_init(ds_ready, 8);
+    mbar_init(all_done, 1);
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t tS = tmem, tP = tmem + 128, tV = tmem + 256, tK = tmem + 256 + D;
+  const int start = next(-1);
+
+  if (warp < 8) {
+    // ------------------------------------------------------------------ scores: a lane a key, `half` of its rows
+    const int half = warp >> 2, key = k0 + (warp & 3) * 32 + lane;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, at = lane_base + (uint32_t)(half * 64);
+    int lo, hi, own = 0;
+    rows_of_keys(p, key, key, prefix, lo, hi);
+    if (key >= p.Tk) hi = -1;
+    if (p.seg_k != nullptr) own = key < p.Tk ? p.seg_k[(long long)b * p.Tk + key] : -1;
+    bool ok = true;
+    int it = 0;
+    for (int g = 0; g < group && ok; ++g) {
+      Lane s;
+      s.f = score_of(p, hkv * group + g);
+      s.cap = p.cap > 0.f;
+      for (int n = start; n < end && ok; n = next(n), ++it) {
+        const int q0 = (first + n) * BLK + half * 64, stage = it % ST;
+        const bool whole = flags[n] & WHOLE;
+        uint32_t keep[2] = {~0u, ~0u};
+        if (!whole) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            keep[c] = span_bits(lo, hi, q0 + c * 32);
+            if (p.seg_q != nullptr) {
+              const int q = q0 + c * 32 + lane;
+              keep[c] &= segment_bits(q < p.Tq ? p.seg_q[(long long)b * p.Tq + q] : -1, own);
+            }
+          }
+        }
+        const float* lse = reinterpret_cast<const float*>(smem_raw + C::SUMS + stage * 1024) + half * 64;
+        ok = mbar_wait(full(stage), (it / ST) & 1, abort_flag) && mbar_wait(s_full, it & 1, abort_flag);
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        float w[64];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float x[32];
+          tmem_ld32(tS + at + (uint32_t)(c * 32), reinterpret_cast<uint32_t*>(x));
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          s.from = (float)(key - q0 - c * 32);
+          probabilities(x, w + c * 32, s, keep[c], whole, [&](int e) { return *reinterpret_cast<const uint64_t*>(lse + c * 32 + e); });
+          uint32_t packed[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) packed[e] = pack_16<T>(x[2 * e], x[2 * e + 1]);
+          tmem_st16(tS + at + (uint32_t)(c * 16), packed);
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready);
+        ok = mbar_wait(dp_full, it & 1, abort_flag);
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float dp[32];
+          tmem_ld32(tP + at + (uint32_t)(c * 32), reinterpret_cast<uint32_t*>(dp));
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          uint32_t packed[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const uint64_t delta2 = *reinterpret_cast<const uint64_t*>(lse + 128 + c * 32 + e);
+            float d0, d1;
+            unpack_f32x2(mul_f32x2(fma_f32x2(delta2, both(-1.f), pack_f32x2(dp[e], dp[e + 1])), pack_f32x2(w[c * 32 + e], w[c * 32 + e + 1])), d0, d1);
+            packed[e / 2] = pack_16<T>(d0, d1);
+          }
+          tmem_st16(tP + at + (uint32_t)(c * 16), packed);
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ds_ready);
+      }
+    }
+    if (ok && it > 0) {
+      ok = __all_sync(0xffffffffu, mbar_wait(all_done, 0, abort_flag));
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    }
+    if (ok) {  // the first four warps store dV, the others dK
+      T* to = (half == 0 ? dv : dk) + (((long long)b * p.Tk + min(key, p.Tk - 1)) * p.Hkv + hkv) * p.D;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) store_row(to, (half == 0 ? tV : tK) + lane_base + (uint32_t)c, c, p.D, half == 0 ? 1.f : p.scale, key < p.Tk, it == 0);
+    } else {
+      if (lane == 0 && err) atomicExch(err, 53);
+      *abort_flag = 1;
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------------------ TMA producer
+    if (elect_one() && start < end) {
+      mbar_expect_tx(kv_bar, 2 * TILE);
+#pragma unroll
+      for (int c = 0; c < C::CH; ++c) {
+        tma_load_4d(sK + c * 16384, &map_k, kv_bar, c * 64, k0, hkv, b);
+        tma_load_4d(sV + c * 16384, &map_v, kv_bar, c * 64, k0, hkv, b);
+      }
+      bool ok = true;
+      int it = 0;
+      for (int g = 0; g < group && ok; ++g) {
+        const int h = hkv * group + g;
+        for (int n = start; n < end; n = next(n), ++it) {
+          const int stage = it % ST, q0 = (first + n) * BLK;
+          ok = mbar_wait(empty(stage), ((it / ST) & 1) ^ 1, abort_flag);
+          if (!ok) break;
+          mbar_expect_tx(full(stage), 2 * TILE + 1024);
+          const uint32_t dst = sQG + stage * C::STAGE;
+#pragma unroll
+          for (int c = 0; c < C::CH; ++c) tma_load_4d(dst + c * 16384, &map_q, full(stage), c * 64, q0, h, b);
+#pragma unroll
+          for (int c = 0; c < C::CH; ++c) tma_load_4d(dst + TILE + c * 16384, &map_g, full(stage), c * 64, q0, h, b);
+          const long long row = ((long long)b * p.H + h) * sums.pitch + q0;
+          const uint32_t to = base + C::SUMS + stage * 1024;
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 512, [%2];" ::"r"(to), "l"(sums.lse + row), "r"(full(stage)) : "memory");
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 512, [%2];" ::"r"(to + 512), "l"(sums.delta + row), "r"(full(stage)) : "memory");
+        }
+      }
+      if (!ok) {
+        if (err) atomicExch(err, 51);
+        *abort_flag = 1;
+        for (uint32_t spin = 0; spin < (1u << 16); ++spin)
+          if (mbar_try_wait(kv_bar, 0)) break;
+        for (int n = max(0, it - ST); n < it; ++n)
+          for (uint32_t spin = 0; spin < (1u << 16); ++spin)
+            if (mbar_try_wait(full(n % ST), (n / ST) & 1)) break;
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ MMA issuer
+    if (elect_one() && start < end) {
+      constexpr uint32_t idesc_s = product_desc<T>(128, 128, false), idesc_o = product_desc<T>(128, D, true);
+      auto rows = [&](uint32_t to, uint32_t a, uint32_t bb) {  // 128 x 128 over the head dimension
+#pragma unroll
+        for (int c = 0; c < C::CH; ++c) {
+          const uint64_t adesc = make_smem_desc(a + c * 16384, false), bdesc = make_smem_desc(bb + c * 16384, false);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_bf16(to, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc_s, (c > 0 || k > 0) ? 1u : 0u);
+        }
+      };
+      auto cols = [&](uint32_t to, uint32_t a, uint32_t bb, bool add) {  // 128 x D over the 128 rows of the tile at bb
+        const uint64_t bdesc = mn_desc(bb, 16384);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          umma_bf16_ts(to, a + (uint32_t)((k >> 2) * 64 + (k & 3) * 8), bdesc + (uint64_t)((2048u >> 4) * k), idesc_o, (add || k > 0) ? 1u : 0u);
+      };
+      int total = 0;
+      for (int n = start; n < end; n = next(n)) ++total;
+      total *= group;
+      auto q_of = [&](int it) { return sQG + (uint32_t)((it % ST) * C::STAGE); };
+      bool ok = mbar_wait(kv_bar, 0, abort_flag) && mbar_wait(full(0), 0, abort_flag);
+      if (ok) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        rows(tS, sK, q_of(0));
+        umma_commit(s_full);
+        rows(tP, sV, q_of(0) + TILE);
+        umma_commit(dp_full);
+      }
+      for (int it = 0; it < total && ok; ++it) {
+        ok = mbar_wait(p_ready, it & 1, abort_flag);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        cols(tV, tS, q_of(it) + TILE, it > 0);
+        if (it + 1 < total) {
+          ok = mbar_wait(full((it + 1) % ST), ((it + 1) / ST) & 1, abort_flag);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          rows(tS, sK, q_of(it + 1));
+          umma_commit(s_full);
+        }
+        ok = mbar_wait(ds_ready, it & 1, abort_flag);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        cols(tK, tP, q_of(it), it > 0);
+        umma_commit(empty(it % ST));
+        if (it + 1 < total) {
+          rows(tP, sV, q_of(it + 1) + TILE);
+          umma_commit(dp_full);
+        }
+      }
+      if (ok) umma_commit(all_done);
+      else {
+        if (err) atomicExch(err, 52);
+        *abort_flag = 1;
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  __syncwarp();
+  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// ------------------------------------------------------------------------------------------------ dQ
+template <int D>
+struct DqCfg {
+  // K is read by the first and by the last product of a tile, V by the one between: three places for K and one for V hold as much as
+  // two of both, and neither is waited for
+  static constexpr int CH = D / 64, TILE = CH * 16384, KS = D == 128 ? 3 : 5, VS = D == 128 ? 1 : 3;
+  static constexpr int BARS = (2 + KS + VS) * TILE, FLAGS = BARS + 256;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(BWD_THREADS, 1)
+rules_dq_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+               const __grid_constant__ CUtensorMap map_g, const Rules p, const Sums sums, T* dq, int* err) {
+  using C = DqCfg<D>;
+  constexpr int TILE = C::TILE, KS = C::KS, VS = C::VS;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t base = smem_u32(smem_raw);
+  if (base & 1023u) {
+    if (threadIdx.x == 0 && err) atomicExch(err, 60);
+    return;
+  }
+  const uint32_t sQ = base, sG = base + TILE, sK = base + 2 * TILE, sV = sK + KS * TILE, bar_base = base + C::BARS;
+  uint8_t* flags = smem_raw + C::FLAGS;
+  const uint32_t q_bar = bar_base, dp_full = bar_base + 8, ds_ready = bar_base + 16, all_done = bar_base + 24;
+  auto s_full = [&](int i) { return bar_base + 32u + 8u * i; };
+  auto k_full = [&](int s) { return bar_base + 48u + 8u * s; };
+  auto k_empty = [&](int s) { return bar_base + 48u + 8u * (KS + s); };
+  auto v_full = [&](int s) { return bar_base + 48u + 8u * (2 * KS + s); };
+  auto v_empty = [&](int s) { return bar_base + 48u + 8u * (2 * KS + VS + s); };
+  static_assert(48 + 16 * (KS + VS) + 8 <= 256, "barrier area");
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem_raw + C::BARS + 48 + 16 * (KS + VS));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int groups = p.H * p.B, n_q = (p.Tq + BLK - 1) / BLK, q0 = (n_q - 1 - (int)(blockIdx.x / groups)) * BLK;
+  const int h = (int)(blockIdx.x % groups) % p.H, b = (int)(blockIdx.x % groups) / p.H, hkv = h / (p.H / p.Hkv);
+  const int prefix = p.prefix != nullptr ? p.prefix[b] : 0;
+  int first, last;  // tiles of keys
+  keys_of_rows(p, q0, min(q0 + BLK, p.Tq) - 1, prefix, first, last);
+  first /= BLK;
+  last = last < 0 ? -1 : last / BLK;
+  for (int n = threadIdx.x; first + n <= last; n += BWD_THREADS) flags[n] = (uint8_t)tile_flags(p, b, q0, (first + n) * BLK, prefix);
+  const int end = last - first + 1;
+  auto next = [&](int n) {
+    do ++n;
+    while (n < end && !(flags[n] & NEEDED));
+    return n;
+  };
+  if (threadIdx.x == 0) {
+    mbar_init(q_bar, 1);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_ready, 8);
+    mbar_init(all_done, 1);
+    mbar_init(s_full(0), 1);
+    mbar_init(s_full(1), 1);
+    for (int s = 0; s < KS; ++s) {
+      mbar_init(k_full(s), 1);
+      mbar_init(k_empty(s), 1);
+    }
+    for (int s = 0; s < VS; ++s) {
+      mbar_init(v_full(s), 1);
+      mbar_init(v_empty(s), 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t tP = tmem + 256, tQ = tmem + 384;
+  const int start = next(-1);
+
+  if (warp < 8) {
+    // ------------------------------------------------------------------ scores: a lane a row, `half` of its keys
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane, qi = q0 + row;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, at = lane_base + (uint32_t)(half * 64);
+    int lo, hi, own = 0;
+    row_span(p, qi, prefix, lo, hi);
+    if (qi >= p.Tq) hi = -1;
+    if (p.seg_q != nullptr) own = qi < p.Tq ? p.seg_q[(long long)b * p.Tq + qi] : -1;
+    const long long sum_at = ((long long)b * p.H + h) * sums.pitch + qi;
+    const uint64_t lse2 = both(sums.lse[sum_at]), minus_delta2 = both(-sums.delta[sum_at]);
+    Lane s;
+    s.f = score_of(p, h);
+    s.cap = p.cap > 0.f;
+    bool ok = true;
+    int it = 0;
+    for (int n = start; n < end; n = next(n), ++it) {
+      const int k0 = (first + n) * BLK + half * 64;
+      const bool whole = flags[n] & WHOLE;
+      const uint32_t tS = tmem + (uint32_t)((it & 1) * 128) + at;
+      uint32_t keep[2] = {~0u, ~0u};
+      if (!whole) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          keep[c] = span_bits(lo, hi, k0 + c * 32);
+          if (p.seg_k != nullptr) {
+            const int k = k0 + c * 32 + lane;
+            keep[c] &= segment_bits(k < p.Tk ? p.seg_k[(long long)b * p.Tk + k] : -1, own);
+          }
+        }
+      }
+      ok = mbar_wait(s_full(it & 1), (it >> 1) & 1, abort_flag);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      float w[64];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float x[32];
+        tmem_ld32(tS + (uint32_t)(c * 32), reinterpret_cast<uint32_t*>(x));
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        s.from = (float)(qi - k0 - c * 32);
+        probabilities(x, w + c * 32, s, keep[c], whole, [&](int) { return lse2; });
+      }
+      ok = mbar_wait(dp_full, it & 1, abort_flag);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float dp[32];
+        tmem_ld32(tP + at + (uint32_t)(c * 32), reinterpret_cast<uint32_t*>(dp));
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        uint32_t packed[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          float d0, d1;
+          unpack_f32x2(mul_f32x2(add_f32x2(pack_f32x2(dp[e], dp[e + 1]), minus_delta2), pack_f32x2(w[c * 32 + e], w[c * 32 + e + 1])), d0, d1);
+          packed[e / 2] = pack_16<T>(d0, d1);
+        }
+        tmem_st16(tS + (uint32_t)(c * 16), packed);
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_ready);
+    }
+    if (ok && it > 0) {
+      ok = __all_sync(0xffffffffu, mbar_wait(all_done, 0, abort_flag));
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    }
+    if (ok) {  // each half of the warps stores half of the columns
+      T* to = dq + (((long long)b * p.Tq + min(qi, p.Tq - 1)) * p.H + h) * p.D;
+#pragma unroll 1
+      for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) store_row(to, tQ + lane_base + (uint32_t)c, c, p.D, p.scale, qi < p.Tq, it == 0);
+    } else {
+      if (lane == 0 && err) atomicExch(err, 63);
+      *abort_flag = 1;
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------------------ TMA producer
+    if (elect_one() && start < end) {
+      mbar_expect_tx(q_bar, 2 * TILE);
+#pragma unroll
+      for (int c = 0; c < C::CH; ++c) {
+        tma_load_4d(sQ + c * 16384, &map_q, q_bar, c * 64, q0, h, b);
+        tma_load_4d(sG + c * 16384, &map_g, q_bar, c * 64, q0, h, b);
+      }
+      bool ok = true;
+      int it_k = 0, it_v = 0;
+      auto load_k = [&](int n) {
+        const int s = it_k % KS;
+        if (!mbar_wait(k_empty(s), ((it_k / KS) & 1) ^ 1, abort_flag)) return false;
+        mbar_expect_tx(k_full(s), TILE);
+#pragma unroll
+        for (int c = 0; c < C::CH; ++c) tma_load_4d(sK + s * TILE + c * 16384, &map_k, k_full(s), c * 64, (first + n) * BLK, hkv, b);
+        ++it_k;
+        return true;
+      };
+      // in the order of the products: K of a tile goes ahead of V of the tile before
+      ok = load_k(start);
+      for (int n = start; n < end && ok;) {
+        const int then = next(n), s = it_v % VS;
+        if (then < end) ok = load_k(then);
+        if (ok) ok = mbar_wait(v_empty(s), ((it_v / VS) & 1) ^ 1, abort_flag);
+        if (!ok) break;
+        mbar_expect_tx(v_full(s), TILE);
+#pragma unroll
+        for (int c = 0; c < C::CH; ++c) tma_load_4d(sV + s * TILE + c * 16384, &map_v, v_full(s), c * 64, (first + n) * BLK, hkv, b);
+        ++it_v;
+        n = then;
+      }
+      if (!ok) {
+        if (err) atomicExch(err, 61);
+        *abort_flag = 1;
+        for (uint32_t spin = 0; spin < (1u << 16); ++spin)
+          if (mbar_try_wait(q_bar, 0)) break;
+        for (int n = max(0, it_k - KS); n < it_k; ++n)
+          for (uint32_t spin = 0; spin < (1u << 16); ++spin)
+            if (mbar_try_wait(k_full(n % KS), (n / KS) & 1)) break;
+        for (int n = max(0, it_v - VS); n < it_v; ++n)
+          for (uint32_t spin = 0; spin < (1u << 16); ++spin)
+            if (mbar_try_wait(v_full(n % VS), (n / VS) & 1)) break;
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ MMA issuer
+    if (elect_one() && start < end) {
+      constexpr uint32_t idesc_s = product_desc<T>(128, 128, false), idesc_o = product_desc<T>(128, D, true);
+      auto rows = [&](uint32_t to, uint32_t a, uint32_t bb) {
+#pragma unroll
+        for (int c = 0; c < C::CH; ++c) {
+          const uint64_t adesc = make_smem_desc(a + c * 16384, false), bdesc = make_smem_desc(bb + c * 16384, false);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_bf16(to, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc_s, (c > 0 || k > 0) ? 1u : 0u);
+        }
+      };
+      auto scores = [&](int it) {
+        const int s = it % KS;
+        if (!mbar_wait(k_full(s), (it / KS) & 1, abort_flag)) return false;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        rows(tmem + (uint32_t)((it & 1) * 128), sQ, sK + s * TILE);
+        umma_commit(s_full(it & 1));
+        return true;
+      };
+      auto grads = [&](int it) {
+        const int s = it % VS;
+        if (!mbar_wait(v_full(s), (it / VS) & 1, abort_flag)) return false;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        rows(tP, sG, sV + s * TILE);
+        umma_commit(dp_full);
+        umma_commit(v_empty(s));
+        return true;
+      };
+      int total = 0;
+      for (int n = start; n < end; n = next(n)) ++total;
+      bool ok = mbar_wait(q_bar, 0, abort_flag) && scores(0) && (total < 2 || scores(1)) && grads(0);
+      for (int it = 0; it < total && ok; ++it) {
+        ok = mbar_wait(ds_ready, it & 1, abort_flag);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t bdesc = mn_desc(sK + (it % KS) * TILE, 16384);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          umma_bf16_ts(tQ, tmem + (uint32_t)((it & 1) * 128 + (k >> 2) * 64 + (k & 3) * 8), bdesc + (uint64_t)((2048u >> 4) * k), idesc_o, (it > 0 || k > 0) ? 1u : 0u);
+        umma_commit(k_empty(it % KS));
+        if (it + 1 < total) ok = grads(it + 1);
+        if (ok && it + 2 < total) ok = scores(it + 2);
+      }
+      if (ok) umma_commit(all_done);
+      else {
+        if (err) atomicExch(err, 62);
+        *abort_flag = 1;
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  __syncwarp();
+  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+int flag_bytes(int T) { return ((T + BLK - 1) / BLK + 15) / 16 * 16; }
+
+template <typename T, int D>
+int launch_bwd(const CUtensorMap* m, const Rules& p, const Sums& sums, void* dq, void* dk, void* dv, int* err, cudaStream_t stream) {
+  static bool attr[2][KB_MAX_DEVICES] = {{false}};
+  if (!kb_allow_smem(rules_dkv_sm100<T, D>, DkvCfg<D>::FLAGS + MAX_BLOCKS, attr[0]) || !kb_allow_smem(rules_dq_sm100<T, D>, DqCfg<D>::FLAGS + MAX_BLOCKS, attr[1])) {
+    kb200_set_error("attention_rules: shared-memory limit");
+    return -3;
+  }
+  if (dk != nullptr)
+    rules_dkv_sm100<T, D><<<(unsigned)((long long)((p.Tk + BLK - 1) / BLK) * p.Hkv * p.B), BWD_THREADS, DkvCfg<D>::FLAGS + flag_bytes(p.Tq), stream>>>(m[0], m[1], m[2], m[3], p,
+                                                                                                                                               sums, (T*)dk, (T*)dv, err);
+  if (dq != nullptr)
+    rules_dq_sm100<T, D><<<(unsigned)((long long)((p.Tq + BLK - 1) / BLK) * p.H * p.B), BWD_THREADS, DqCfg<D>::FLAGS + flag_bytes(p.Tk), stream>>>(m[0], m[1], m[2], m[3], p, sums,
+                                                                                                                                           (T*)dq, err);
+  return 0;
+}
+
+}  // namespace
+
+// As kb200_attention_rules_bwd for what kb200_attention_rules_fwd_sm100 takes, at most 1048576 rows and keys; lse and delta with rows `pitch` apart, a
+// multiple of 128.
+KB_API int kb200_attention_rules_bwd_sm100(const void* q, const void* k, const void* v, const void* grad_out, const long long* strides, const float* lse, const float* delta,
+                                           int pitch, void* dq, void* dk, void* dv, int dtype, int B, int H, int Hkv, int Tq, int Tk, int D, int* err, float scale, float cap,
+                                           const float* slopes, int causal, int window, const int* prefix, const int* seg_q, const int* seg_k, const void* range_q,
+                                           const void* range_k, cudaStream_t stream) {
+  const Rules p{B, H, Hkv, Tq, Tk, D, scale, cap, slopes, causal, window, prefix, seg_q, seg_k, (const int4*)range_q, (const int4*)range_k};
+  if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || Tq <= 0 || Tk <= 0 || D <= 0 || D > 128 || D % 8 || (dtype != 1 && dtype != 2) || Tk > MAX_BLOCKS * BLK ||
+      Tq > MAX_BLOCKS * BLK || pitch % BLK || pitch < Tq || (long long)((Tq + 127) / 128) * H * B > 0x7fffffffll || (long long)((Tk + 127) / 128) * Hkv * B > 0x7fffffffll) {
+    kb200_set_error("attention_rules_bwd_sm100: sizes out of range");
+    return -2;
+  }
+  const Strides qs{strides[0], strides[1], strides[2]}, ks{strides[3], strides[4], strides[5]}, vs{strides[6], strides[7], strides[8]}, gs{strides[9], strides[10], strides[11]};
+  if (!rules_strides(qs, q, Tq, H, B) || !rules_strides(ks, k, Tk, Hkv, B) || !rules_strides(vs, v, Tk, Hkv, B) || !rules_strides(gs, grad_out, Tq, H, B) ||
+      (((uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)lse | (uintptr_t)delta) & 15)) {
+    kb200_set_error("attention_rules_bwd_sm100: strides and base pointers must be multiples of 16 bytes");
+    return -2;
+  }
+  const bool half = dtype == 2;
+  CUtensorMap m[4];
+  if (!rules_map(&m[0], q, D, Tq, H, B, qs, 128, half) || !rules_map(&m[1], k, D, Tk, Hkv, B, ks, 128, half) || !rules_map(&m[2], v, D, Tk, Hkv, B, vs, 128, half) ||
+      !rules_map(&m[3], grad_out, D, Tq, H, B, gs, 128, half)) {
+    kb200_set_error("attention_rules_bwd_sm100: cuTensorMapEncodeTiled failed");
+    return -3;
+  }
+  const Sums sums{lse, delta, pitch};
+  int rc;
+  if (D <= 64) rc = half ? launch_bwd<__half, 64>(m, p, sums, dq, dk, dv, err, stream) : launch_bwd<__nv_bfloat16, 64>(m, p, sums, dq, dk, dv, err, stream);
+  else rc = half ? launch_bwd<__half, 128>(m, p, sums, dq, dk, dv, err, stream) : launch_bwd<__nv_bfloat16, 128>(m, p, sums, dq, dk, dv, err, stream);
+  if (rc != 0) return rc;
+  KB_CHECK_LAUNCH("attention_rules_bwd_sm100");
+  return 0;
+}

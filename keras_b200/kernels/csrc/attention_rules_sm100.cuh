@@ -1,0 +1,128 @@
+// What the tensor-core kernels of attention by rules share: which tiles of 128 x 128 pairs have to be looked at, and the scores of a thread's
+// part of one.  attention_rules.cuh says what a score is and which keys a row sees.
+#pragma once
+#include "attention_rules.cuh"
+#include "attention_sm100.cuh"
+
+namespace kbrules {
+using namespace kbgemm;
+using namespace kbattn;
+
+constexpr int BLK = 128;
+constexpr int MAX_BLOCKS = 8192;  // tiles of keys (or rows) that one CTA's flags hold: 1048576 positions
+enum { NEEDED = 1, WHOLE = 2 };   // flags of a pair of tiles: some pair is visible; every pair is
+
+// Flags of rows i0 .. i0 + 127 against keys k0 .. k0 + 127.
+__device__ __forceinline__ int tile_flags(const Rules& r, int b, int i0, int k0, int prefix) {
+  const int i1 = min(i0 + BLK, r.Tq) - 1, k1 = min(k0 + BLK, r.Tk) - 1;
+  if (i1 < i0 || k1 < k0) return 0;
+  int lo, hi;
+  keys_of_rows(r, i0, i1, prefix, lo, hi);
+  if (k0 > hi || k1 < lo || !segments_meet(r, b, i0, k0)) return 0;
+  bool whole = k0 + BLK <= r.Tk && segments_same(r, b, i0, k0);
+  if (r.causal && k1 > i0 && k1 >= prefix) whole = false;
+  if (r.window > 0 && (i1 - k0 >= r.window || k1 - i0 >= r.window)) whole = false;
+  return NEEDED | (whole ? WHOLE : 0);
+}
+
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t both(float a) { return pack_f32x2(a, a); }
+
+// tanh of two values of at most 1: x times a polynomial of degree 5 in x^2, fitted as tanh_small's (7e-7 of the value with its roundings, a
+// thousandth of what rounding the probabilities to 16 bits costs under a cap of 50).
+__device__ __forceinline__ uint64_t tanh_small2(uint64_t x) {
+  const uint64_t u = mul_f32x2(x, x);
+  uint64_t p = fma_f32x2(both(-0.0030670708511024714f), u, both(0.016743140295147896f));
+  p = fma_f32x2(p, u, both(-0.051605693995952606f));
+  p = fma_f32x2(p, u, both(0.13281434774398804f));
+  p = fma_f32x2(p, u, both(-0.3332904279232025f));
+  p = fma_f32x2(p, u, both(0.9999994039535522f));
+  return mul_f32x2(p, x);
+}
+
+// x[e] := tanh(x[e] * pre), for a warp: on the FMA pipe as long as no lane has a value beyond 1.
+template <int N>
+__device__ __forceinline__ void capped(float (&x)[N], float pre) {
+  const uint64_t pre2 = both(pre);
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < N; e += 2) {
+    unpack_f32x2(mul_f32x2(pack_f32x2(x[e], x[e + 1]), pre2), x[e], x[e + 1]);
+    top = fmaxf(top, fmaxf(fabsf(x[e]), fabsf(x[e + 1])));
+  }
+  if (__any_sync(0xffffffffu, top > 1.f)) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = tanh_any(x[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) unpack_f32x2(tanh_small2(pack_f32x2(x[e], x[e + 1])), x[e], x[e + 1]);
+  }
+}
+
+// Bits of the elements e of 32 with lo <= at + e <= hi.
+__device__ __forceinline__ uint32_t span_bits(int lo, int hi, int at) {
+  const int a = lo - at, z = hi - at;
+  if (z < 0 || a > 31 || z < a) return 0;
+  return (0xffffffffu >> (31 - min(z, 31))) & (0xffffffffu << max(a, 0));
+}
+// Bits of the elements whose segment is the lane's own; `id`: the segment of element `lane`.
+__device__ __forceinline__ uint32_t segment_bits(int id, int own) {
+  const int lo = __reduce_min_sync(0xffffffffu, id), hi = __reduce_max_sync(0xffffffffu, id);
+  if (lo == hi) return lo == own && own >= 0 ? 0xffffffffu : 0u;
+  uint32_t bits = 0;
+#pragma unroll
+  for (int e = 0; e < 32; ++e) bits |= (__shfl_sync(0xffffffffu, id, e) == own ? 1u : 0u) << e;
+  return own >= 0 ? bits : 0u;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack_16(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack_16<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack_16<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename T>
+__device__ __forceinline__ void unpack_16(uint32_t w, float& a, float& b);
+template <>
+__device__ __forceinline__ void unpack_16<__nv_bfloat16>(uint32_t w, float& a, float& b) {
+  a = __uint_as_float(w << 16);
+  b = __uint_as_float(w & 0xffff0000u);
+}
+template <>
+__device__ __forceinline__ void unpack_16<__half>(uint32_t w, float& a, float& b) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  a = f.x;
+  b = f.y;
+}
+
+// Instruction descriptor of a product of 16-bit operands with float32 sums: M x N, B's major direction.
+template <typename T>
+constexpr uint32_t product_desc(int m, int n, bool b_mn_major) {
+  const uint32_t bf16 = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1u : 0u;
+  return (1u << 4) | (bf16 << 7) | (bf16 << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// Operand of rows of 64 values (128 bytes, swizzled), read along the rows' direction; the next 64 values `next` bytes further.
+__device__ __forceinline__ uint64_t mn_desc(uint32_t addr, uint32_t next) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(next >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// Tensor map of a [B, T, H, D] tensor; a dimension of one element has no stride to speak of.
+static inline bool rules_map(CUtensorMap* map, const void* p, int D, int T, int H, int B, const Strides& s, int box_t, bool half) {
+  return make_map_bthd(map, p, D, T, H, B, T == 1 ? 8 : s.t, H == 1 ? 8 : s.h, B == 1 ? 8 : s.b, 64, box_t, half);
+}
+static inline bool rules_strides(const Strides& s, const void* p, int T, int H, int B) {
+  auto ok = [](long long v, int n) { return n == 1 || (v > 0 && v % 8 == 0 && v < (1ll << 38)); };
+  return ok(s.t, T) && ok(s.h, H) && ok(s.b, B) && ((uintptr_t)p & 15) == 0;
+}
+
+}  // namespace kbrules

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import keras_b200 as keras
-from keras_b200.kernels import attention_cache, attention_rules, ops as kops
+from keras_b200.kernels import attention, attention_cache, attention_rules, ops as kops
 from tests import attention_definition as definition
 from tests.test_attention_rules import SLOPES, _Decoder, _generation
 
@@ -153,6 +153,12 @@ def test_scores_beyond_the_cap_and_scales_of_any_sign(dtype):
         found = _definition(q, k, v, do, dict(sliding_window=50), scale=scale)
         for name, got in zip(("out", "dq", "dk", "dv"), _run(q, k, v, do, dict(sliding_window=50, scale=scale))):
             definition.check(name, got, found)
+
+
+@pytest.fixture(autouse=True)
+def _no_wait_ran_out():
+    yield
+    attention.check_errors()
 
 
 @pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.float32, 64), (torch.float16, 128)])
@@ -493,7 +499,13 @@ def test_refusals_of_the_entries():
     assert attention_rules.attention(big, big, big, rules, None) is None
     assert attention_cache.attention(big, big, big, big, big, torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda"), 1.0, None,
                                      None, None) is None
-    fn = attention_rules.launcher("kb200_attention_rules_fwd", [attention_rules._V] * 6 + [attention_rules._I] * 7 + attention_rules._RULES)
+    V, I = attention_rules._V, attention_rules._I
+    fn = attention_rules.launcher("kb200_attention_rules_fwd", [V] * 5 + [I, V] + [I] * 7 + attention_rules._RULES)
     out = torch.empty_like(q)
-    code = fn(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None, attention_rules.strides(q, k, v), 0, 1, 2, 2, 4, 4, 300, *attention_rules._tail(rules, (None, None)))
-    assert code == -2 and lib is not None
+    at = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr())
+    tail = attention_rules._tail(rules, (None, None))
+    assert fn(*at, None, 128, attention_rules.strides(q, k, v), 0, 1, 2, 2, 4, 4, 300, *tail) == -2 and lib is not None
+    fn = attention_rules.launcher("kb200_attention_rules_fwd_sm100", [V] * 6 + [I, V] + [I] * 7 + [V] + attention_rules._RULES)
+    assert fn(*at, None, None, 128, attention_rules.strides(q, k, v), 0, 1, 2, 2, 4, 4, 64, None, *tail) == -2  # float32
+    assert fn(*at, None, None, 128, attention_rules.strides(q, k, v), 1, 1, 2, 2, 4, 4, 60, None, *tail) == -2
+    assert fn(at[0] + 2, *at[1:], None, None, 128, attention_rules.strides(q, k, v), 1, 1, 2, 2, 4, 4, 64, None, *tail) == -2
