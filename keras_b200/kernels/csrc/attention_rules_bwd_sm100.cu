@@ -6,7 +6,7 @@
 //   rules_dq   a CTA a tile of 128 rows; walks over the tiles of keys.
 //              S = Q K^T (two buffers), dP = dO V^T, dS back to TMEM as the operand of dQ += dS K
 //
-// Eight warps work on the scores: two threads a TMEM lane, each with 64 of its 128 columns, so that neither needs a shuffle.  With the lane
+// Sixteen warps work on the scores: four threads a TMEM lane, each with 32 of its 128 columns, so that none needs a shuffle.  With the lane
 // a key (dkv) or a row (dq), every operand is a tile as TMA brought it: the same tile is read along its rows for one product and across
 // them for the other.  Products run in issue order: S of the next tile may be queued behind the product that reads P from the same columns,
 // while the threads are still busy with dS.
@@ -24,37 +24,31 @@ struct Sums {
   int pitch;
 };
 
-// From 32 raw scores (columns e of a lane) to probabilities x and w = P (1 - tanh^2).  `from - e` is the distance of the pair.
-struct Lane {
-  Score f;
-  bool cap;
-  float from;
-};
+// From 32 raw scores (columns e of a lane) to probabilities x and w = P (1 - tanh^2).  `from` - e is the distance of the pair; minus_lse(e): of
+// columns e and e + 1.
 template <typename Lse>
-__device__ __forceinline__ void probabilities(float (&x)[32], float* w, const Lane& s, uint32_t keep, bool whole, Lse lse2) {
-  if (s.cap) {
-    capped(x, s.f.pre);
-    const uint64_t post2 = both(s.f.post);
+__device__ __forceinline__ void probabilities(float (&x)[32], float (&w)[32], const Score& f, bool cap, const Cap& c, float from, uint32_t keep, bool whole, Lse minus_lse) {
+  const bool folded = !cap && f.slope == 0.f;
+  scores32(x, cap, c, folded ? 1.f : f.post, f.slope, from);
+  if (cap) {
+    const uint64_t inv2 = both(-c.inv_post * c.inv_post);
+    if (f.slope == 0.f) {
 #pragma unroll
-    for (int e = 0; e < 32; e += 2) {
-      const uint64_t t = pack_f32x2(x[e], x[e + 1]);
-      unpack_f32x2(fma_f32x2(mul_f32x2(t, both(-1.f)), t, both(1.f)), w[e], w[e + 1]);
-      unpack_f32x2(mul_f32x2(t, post2), x[e], x[e + 1]);
+      for (int e = 0; e < 32; e += 2) {
+        const uint64_t t = pack_f32x2(x[e], x[e + 1]);
+        unpack_f32x2(fma_f32x2(mul_f32x2(t, inv2), t, both(1.f)), w[e], w[e + 1]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {  // the score without its distance
+        const float t = fmaf(f.slope, fabsf(from - (float)e), x[e]) * c.inv_post;
+        w[e] = fmaf(-t, t, 1.f);
+      }
     }
   }
-  const uint64_t scale2 = both(s.cap ? 1.f : s.f.post);
-  if (s.f.slope != 0.f) {
+  const uint64_t scale2 = both(folded ? f.post : 1.f);
 #pragma unroll
-    for (int e = 0; e < 32; e += 2) {
-      unpack_f32x2(mul_f32x2(pack_f32x2(x[e], x[e + 1]), scale2), x[e], x[e + 1]);
-      x[e] = fmaf(-s.f.slope, fabsf(s.from - (float)e), x[e]);
-      x[e + 1] = fmaf(-s.f.slope, fabsf(s.from - (float)(e + 1)), x[e + 1]);
-      unpack_f32x2(add_f32x2(pack_f32x2(x[e], x[e + 1]), mul_f32x2(lse2(e), both(-1.f))), x[e], x[e + 1]);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 32; e += 2) unpack_f32x2(fma_f32x2(pack_f32x2(x[e], x[e + 1]), scale2, mul_f32x2(lse2(e), both(-1.f))), x[e], x[e + 1]);
-  }
+  for (int e = 0; e < 32; e += 2) unpack_f32x2(fma_f32x2(pack_f32x2(x[e], x[e + 1]), scale2, minus_lse(e)), x[e], x[e + 1]);
   if (!whole) {
 #pragma unroll
     for (int e = 0; e < 32; ++e)
@@ -63,7 +57,7 @@ __device__ __forceinline__ void probabilities(float (&x)[32], float* w, const La
 #pragma unroll
   for (int e = 0; e < 32; ++e) {
     x[e] = ex2(x[e]);
-    w[e] = s.cap ? w[e] * x[e] : x[e];
+    w[e] = cap ? w[e] * x[e] : x[e];
   }
 }
 
@@ -84,7 +78,7 @@ __device__ __forceinline__ void store_row(T* to, uint32_t tmem, int col, int D, 
   }
 }
 
-constexpr int BWD_THREADS = 320;
+constexpr int BWD_THREADS = 576;  // 16 warps on the scores, one for copies, one for products
 
 // ------------------------------------------------------------------------------------------------ dK, dV
 template <int D>
@@ -96,7 +90,7 @@ struct DkvCfg {
 template <typename T, int D>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
 rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                const __grid_constant__ CUtensorMap map_g, const Rules p, const Sums sums, T* dk, T* dv, int* err) {
+                const __grid_constant__ CUtensorMap map_g, const Rules p, const Cap c_, const Sums sums, T* dk, T* dv, int* err) {
   using C = DkvCfg<D>;
   constexpr int TILE = C::TILE, ST = C::STAGES;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -132,8 +126,8 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     mbar_init(kv_bar, 1);
     mbar_init(s_full, 1);
     mbar_init(dp_full, 1);
-    mbar_init(p_ready, 8);
-    mbar_init(ds_ready, 8);
+    mbar_init(p_ready, 16);
+    mbar_init(ds_ready, 16);
     mbar_init(all_done, 1);
     for (int s = 0; s < ST; ++s) {
       mbar_init(full(s), 1);
@@ -142,7 +136,7 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 9) {
+  if (warp == 17) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -153,10 +147,11 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const uint32_t tS = tmem, tP = tmem + 128, tV = tmem + 256, tK = tmem + 256 + D;
   const int start = next(-1);
 
-  if (warp < 8) {
-    // ------------------------------------------------------------------ scores: a lane a key, `half` of its rows
-    const int half = warp >> 2, key = k0 + (warp & 3) * 32 + lane;
-    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, at = lane_base + (uint32_t)(half * 64);
+  if (warp < 16) {
+    // ------------------------------------------------------------------ scores: a lane a key, 32 of its rows
+    const int part = warp >> 2, key = k0 + (warp & 3) * 32 + lane;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, at = lane_base + (uint32_t)(part * 32);
+    const bool cap = p.cap > 0.f;
     int lo, hi, own = 0;
     rows_of_keys(p, key, key, prefix, lo, hi);
     if (key >= p.Tk) hi = -1;
@@ -164,40 +159,27 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     bool ok = true;
     int it = 0;
     for (int g = 0; g < group && ok; ++g) {
-      Lane s;
-      s.f = score_of(p, hkv * group + g);
-      s.cap = p.cap > 0.f;
-      for (int n = start; n < end && ok; n = next(n), ++it) {
-        const int q0 = (first + n) * BLK + half * 64, stage = it % ST;
+      const Score f = score_of(p, hkv * group + g);
+      for (int n = start; n < end; n = next(n), ++it) {
+        const int q0 = (first + n) * BLK + part * 32, stage = it % ST;
         const bool whole = flags[n] & WHOLE;
-        uint32_t keep[2] = {~0u, ~0u};
+        uint32_t keep = ~0u;
         if (!whole) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            keep[c] = span_bits(lo, hi, q0 + c * 32);
-            if (p.seg_q != nullptr) {
-              const int q = q0 + c * 32 + lane;
-              keep[c] &= segment_bits(q < p.Tq ? p.seg_q[(long long)b * p.Tq + q] : -1, own);
-            }
-          }
+          keep = span_bits(lo, hi, q0);
+          if (p.seg_q != nullptr) keep &= segment_bits(q0 + lane < p.Tq ? p.seg_q[(long long)b * p.Tq + q0 + lane] : -1, own);
         }
-        const float* lse = reinterpret_cast<const float*>(smem_raw + C::SUMS + stage * 1024) + half * 64;
+        const float* lse = reinterpret_cast<const float*>(smem_raw + C::SUMS + stage * 1024) + part * 32;
         ok = mbar_wait(full(stage), (it / ST) & 1, abort_flag) && mbar_wait(s_full, it & 1, abort_flag);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        float w[64];
+        float x[32], w[32];
+        tmem_ld32(tS + at, reinterpret_cast<uint32_t*>(x));
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        probabilities(x, w, f, cap, c_, (float)(key - q0), keep, whole, [&](int e) { return mul_f32x2(*reinterpret_cast<const uint64_t*>(lse + e), both(-1.f)); });
+        uint32_t packed[16];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float x[32];
-          tmem_ld32(tS + at + (uint32_t)(c * 32), reinterpret_cast<uint32_t*>(x));
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-          s.from = (float)(key - q0 - c * 32);
-          probabilities(x, w + c * 32, s, keep[c], whole, [&](int e) { return *reinterpret_cast<const uint64_t*>(lse + c * 32 + e); });
-          uint32_t packed[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) packed[e] = pack_16<T>(x[2 * e], x[2 * e + 1]);
-          tmem_st16(tS + at + (uint32_t)(c * 16), packed);
-        }
+        for (int e = 0; e < 16; ++e) packed[e] = pack_16<T>(x[2 * e], x[2 * e + 1]);
+        tmem_st16(tS + at, packed);
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
@@ -205,21 +187,16 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         ok = mbar_wait(dp_full, it & 1, abort_flag);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        tmem_ld32(tP + at, reinterpret_cast<uint32_t*>(x));
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float dp[32];
-          tmem_ld32(tP + at + (uint32_t)(c * 32), reinterpret_cast<uint32_t*>(dp));
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-          uint32_t packed[16];
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const uint64_t delta2 = *reinterpret_cast<const uint64_t*>(lse + 128 + c * 32 + e);
-            float d0, d1;
-            unpack_f32x2(mul_f32x2(fma_f32x2(delta2, both(-1.f), pack_f32x2(dp[e], dp[e + 1])), pack_f32x2(w[c * 32 + e], w[c * 32 + e + 1])), d0, d1);
-            packed[e / 2] = pack_16<T>(d0, d1);
-          }
-          tmem_st16(tP + at + (uint32_t)(c * 16), packed);
+        for (int e = 0; e < 32; e += 2) {
+          const uint64_t delta2 = *reinterpret_cast<const uint64_t*>(lse + 128 + e);
+          float d0, d1;
+          unpack_f32x2(mul_f32x2(fma_f32x2(delta2, both(-1.f), pack_f32x2(x[e], x[e + 1])), pack_f32x2(w[e], w[e + 1])), d0, d1);
+          packed[e / 2] = pack_16<T>(d0, d1);
         }
+        tmem_st16(tP + at, packed);
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
@@ -230,15 +207,16 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       ok = __all_sync(0xffffffffu, mbar_wait(all_done, 0, abort_flag));
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     }
-    if (ok) {  // the first four warps store dV, the others dK
-      T* to = (half == 0 ? dv : dk) + (((long long)b * p.Tk + min(key, p.Tk - 1)) * p.Hkv + hkv) * p.D;
+    if (ok) {  // half of the warps store dV, the others dK, each half of the columns
+      T* to = (part < 2 ? dv : dk) + (((long long)b * p.Tk + min(key, p.Tk - 1)) * p.Hkv + hkv) * p.D;
 #pragma unroll 1
-      for (int c = 0; c < D; c += 32) store_row(to, (half == 0 ? tV : tK) + lane_base + (uint32_t)c, c, p.D, half == 0 ? 1.f : p.scale, key < p.Tk, it == 0);
+      for (int c = (part & 1) * (D / 2); c < ((part & 1) + 1) * (D / 2); c += 32)
+        store_row(to, (part < 2 ? tV : tK) + lane_base + (uint32_t)c, c, p.D, part < 2 ? 1.f : p.scale, key < p.Tk, it == 0);
     } else {
       if (lane == 0 && err) atomicExch(err, 53);
       *abort_flag = 1;
     }
-  } else if (warp == 8) {
+  } else if (warp == 16) {
     // ------------------------------------------------------------------ TMA producer
     if (elect_one() && start < end) {
       mbar_expect_tx(kv_bar, 2 * TILE);
@@ -293,7 +271,7 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         const uint64_t bdesc = mn_desc(bb, 16384);
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          umma_bf16_ts(to, a + (uint32_t)((k >> 2) * 64 + (k & 3) * 8), bdesc + (uint64_t)((2048u >> 4) * k), idesc_o, (add || k > 0) ? 1u : 0u);
+          umma_bf16_ts(to, a + (uint32_t)((k >> 1) * 32 + (k & 1) * 8), bdesc + (uint64_t)((2048u >> 4) * k), idesc_o, (add || k > 0) ? 1u : 0u);
       };
       int total = 0;
       for (int n = start; n < end; n = next(n)) ++total;
@@ -339,7 +317,7 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   __syncwarp();
-  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (warp == 17) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 // ------------------------------------------------------------------------------------------------ dQ
@@ -354,7 +332,7 @@ struct DqCfg {
 template <typename T, int D>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
 rules_dq_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-               const __grid_constant__ CUtensorMap map_g, const Rules p, const Sums sums, T* dq, int* err) {
+               const __grid_constant__ CUtensorMap map_g, const Rules p, const Cap c_, const Sums sums, T* dq, int* err) {
   using C = DqCfg<D>;
   constexpr int TILE = C::TILE, KS = C::KS, VS = C::VS;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -393,7 +371,7 @@ rules_dq_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   if (threadIdx.x == 0) {
     mbar_init(q_bar, 1);
     mbar_init(dp_full, 1);
-    mbar_init(ds_ready, 8);
+    mbar_init(ds_ready, 16);
     mbar_init(all_done, 1);
     mbar_init(s_full(0), 1);
     mbar_init(s_full(1), 1);
@@ -408,7 +386,7 @@ rules_dq_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 9) {
+  if (warp == 17) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -419,65 +397,49 @@ rules_dq_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   const uint32_t tP = tmem + 256, tQ = tmem + 384;
   const int start = next(-1);
 
-  if (warp < 8) {
-    // ------------------------------------------------------------------ scores: a lane a row, `half` of its keys
-    const int half = warp >> 2, row = (warp & 3) * 32 + lane, qi = q0 + row;
-    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, at = lane_base + (uint32_t)(half * 64);
+  if (warp < 16) {
+    // ------------------------------------------------------------------ scores: a lane a row, 32 of its keys
+    const int part = warp >> 2, row = (warp & 3) * 32 + lane, qi = q0 + row;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, at = lane_base + (uint32_t)(part * 32);
+    const bool cap = p.cap > 0.f;
+    const Score f = score_of(p, h);
     int lo, hi, own = 0;
     row_span(p, qi, prefix, lo, hi);
     if (qi >= p.Tq) hi = -1;
     if (p.seg_q != nullptr) own = qi < p.Tq ? p.seg_q[(long long)b * p.Tq + qi] : -1;
     const long long sum_at = ((long long)b * p.H + h) * sums.pitch + qi;
-    const uint64_t lse2 = both(sums.lse[sum_at]), minus_delta2 = both(-sums.delta[sum_at]);
-    Lane s;
-    s.f = score_of(p, h);
-    s.cap = p.cap > 0.f;
+    const uint64_t minus_lse2 = both(-sums.lse[sum_at]), minus_delta2 = both(-sums.delta[sum_at]);
     bool ok = true;
     int it = 0;
     for (int n = start; n < end; n = next(n), ++it) {
-      const int k0 = (first + n) * BLK + half * 64;
+      const int k0 = (first + n) * BLK + part * 32;
       const bool whole = flags[n] & WHOLE;
       const uint32_t tS = tmem + (uint32_t)((it & 1) * 128) + at;
-      uint32_t keep[2] = {~0u, ~0u};
+      uint32_t keep = ~0u;
       if (!whole) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          keep[c] = span_bits(lo, hi, k0 + c * 32);
-          if (p.seg_k != nullptr) {
-            const int k = k0 + c * 32 + lane;
-            keep[c] &= segment_bits(k < p.Tk ? p.seg_k[(long long)b * p.Tk + k] : -1, own);
-          }
-        }
+        keep = span_bits(lo, hi, k0);
+        if (p.seg_k != nullptr) keep &= segment_bits(k0 + lane < p.Tk ? p.seg_k[(long long)b * p.Tk + k0 + lane] : -1, own);
       }
       ok = mbar_wait(s_full(it & 1), (it >> 1) & 1, abort_flag);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      float w[64];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float x[32];
-        tmem_ld32(tS + (uint32_t)(c * 32), reinterpret_cast<uint32_t*>(x));
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        s.from = (float)(qi - k0 - c * 32);
-        probabilities(x, w + c * 32, s, keep[c], whole, [&](int) { return lse2; });
-      }
+      float x[32], w[32];
+      tmem_ld32(tS, reinterpret_cast<uint32_t*>(x));
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      probabilities(x, w, f, cap, c_, (float)(qi - k0), keep, whole, [&](int) { return minus_lse2; });
       ok = mbar_wait(dp_full, it & 1, abort_flag);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      tmem_ld32(tP + at, reinterpret_cast<uint32_t*>(x));
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      uint32_t packed[16];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float dp[32];
-        tmem_ld32(tP + at + (uint32_t)(c * 32), reinterpret_cast<uint32_t*>(dp));
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        uint32_t packed[16];
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          float d0, d1;
-          unpack_f32x2(mul_f32x2(add_f32x2(pack_f32x2(dp[e], dp[e + 1]), minus_delta2), pack_f32x2(w[c * 32 + e], w[c * 32 + e + 1])), d0, d1);
-          packed[e / 2] = pack_16<T>(d0, d1);
-        }
-        tmem_st16(tS + (uint32_t)(c * 16), packed);
+      for (int e = 0; e < 32; e += 2) {
+        float d0, d1;
+        unpack_f32x2(mul_f32x2(add_f32x2(pack_f32x2(x[e], x[e + 1]), minus_delta2), pack_f32x2(w[e], w[e + 1])), d0, d1);
+        packed[e / 2] = pack_16<T>(d0, d1);
       }
+      tmem_st16(tS, packed);
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -487,15 +449,14 @@ rules_dq_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       ok = __all_sync(0xffffffffu, mbar_wait(all_done, 0, abort_flag));
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     }
-    if (ok) {  // each half of the warps stores half of the columns
+    if (ok) {  // a quarter of the warps for every 32 columns
       T* to = dq + (((long long)b * p.Tq + min(qi, p.Tq - 1)) * p.H + h) * p.D;
-#pragma unroll 1
-      for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) store_row(to, tQ + lane_base + (uint32_t)c, c, p.D, p.scale, qi < p.Tq, it == 0);
+      if (part * 32 < D) store_row(to, tQ + lane_base + (uint32_t)(part * 32), part * 32, p.D, p.scale, qi < p.Tq, it == 0);
     } else {
       if (lane == 0 && err) atomicExch(err, 63);
       *abort_flag = 1;
     }
-  } else if (warp == 8) {
+  } else if (warp == 16) {
     // ------------------------------------------------------------------ TMA producer
     if (elect_one() && start < end) {
       mbar_expect_tx(q_bar, 2 * TILE);
@@ -580,7 +541,7 @@ rules_dq_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         const uint64_t bdesc = mn_desc(sK + (it % KS) * TILE, 16384);
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          umma_bf16_ts(tQ, tmem + (uint32_t)((it & 1) * 128 + (k >> 2) * 64 + (k & 3) * 8), bdesc + (uint64_t)((2048u >> 4) * k), idesc_o, (it > 0 || k > 0) ? 1u : 0u);
+          umma_bf16_ts(tQ, tmem + (uint32_t)((it & 1) * 128 + (k >> 1) * 32 + (k & 1) * 8), bdesc + (uint64_t)((2048u >> 4) * k), idesc_o, (it > 0 || k > 0) ? 1u : 0u);
         umma_commit(k_empty(it % KS));
         if (it + 1 < total) ok = grads(it + 1);
         if (ok && it + 2 < total) ok = scores(it + 2);
@@ -595,7 +556,7 @@ rules_dq_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   __syncwarp();
-  if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (warp == 17) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 int flag_bytes(int T) { return ((T + BLK - 1) / BLK + 15) / 16 * 16; }
@@ -607,11 +568,12 @@ int launch_bwd(const CUtensorMap* m, const Rules& p, const Sums& sums, void* dq,
     kb200_set_error("attention_rules: shared-memory limit");
     return -3;
   }
+  const Cap cap = make_cap(p.scale, p.cap);
   if (dk != nullptr)
-    rules_dkv_sm100<T, D><<<(unsigned)((long long)((p.Tk + BLK - 1) / BLK) * p.Hkv * p.B), BWD_THREADS, DkvCfg<D>::FLAGS + flag_bytes(p.Tq), stream>>>(m[0], m[1], m[2], m[3], p,
+    rules_dkv_sm100<T, D><<<(unsigned)((long long)((p.Tk + BLK - 1) / BLK) * p.Hkv * p.B), BWD_THREADS, DkvCfg<D>::FLAGS + flag_bytes(p.Tq), stream>>>(m[0], m[1], m[2], m[3], p, cap,
                                                                                                                                                sums, (T*)dk, (T*)dv, err);
   if (dq != nullptr)
-    rules_dq_sm100<T, D><<<(unsigned)((long long)((p.Tq + BLK - 1) / BLK) * p.H * p.B), BWD_THREADS, DqCfg<D>::FLAGS + flag_bytes(p.Tk), stream>>>(m[0], m[1], m[2], m[3], p, sums,
+    rules_dq_sm100<T, D><<<(unsigned)((long long)((p.Tq + BLK - 1) / BLK) * p.H * p.B), BWD_THREADS, DqCfg<D>::FLAGS + flag_bytes(p.Tk), stream>>>(m[0], m[1], m[2], m[3], p, cap, sums,
                                                                                                                                            (T*)dq, err);
   return 0;
 }

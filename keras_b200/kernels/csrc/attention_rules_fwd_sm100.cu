@@ -25,17 +25,19 @@ struct FwdCfg {
   static constexpr int TILE = CH * 16384;
   static constexpr int RING = NT == 2 ? (D == 128 ? 4 : 8) : (D == 128 ? 2 : 4);
   static constexpr int BARS = (NT + RING) * TILE;
-  static constexpr int FLAGS = BARS + 256;
+  static constexpr int FLAGS = BARS + 384 + 2 * NT * 2 * 128 * 4;
   static constexpr int SMEM = FLAGS;  // and a byte a tile of keys
   static constexpr uint32_t TMEM_COLS = NT == 2 ? 512 : 256;
-  static constexpr int THREADS_ = NT == 2 ? 384 : 192;
+  static constexpr int SOFTMAX = 8 * NT;                 // warps: two threads a row
+  static constexpr int THREADS_ = (SOFTMAX + 2) * 32;
+  static constexpr int EXCHANGE = BARS + 384;            // [parity][tile][half][row] maxima
 };
 constexpr float RESCALE = 8.f;
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(FwdCfg<D, NT>::THREADS_, NT == 2 ? 1 : 2)
 rules_fwd_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                const __grid_constant__ CUtensorMap map_o, const __grid_constant__ CUtensorMap map_lo, const Rules p, float* lse, int pitch, int with_lo, int* err) {
+                const Rules p, const Cap c_, T* o, T* lo_out, float* lse, int pitch, int* err) {
   using C = FwdCfg<D, NT>;
   constexpr int TILE = C::TILE, RING = C::RING;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -50,10 +52,11 @@ rules_fwd_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   auto kv_full = [&](int s) { return bar_base + 8u * (1 + s); };
   auto kv_empty = [&](int s) { return bar_base + 8u * (1 + RING + s); };
   auto s_full = [&](int i) { return bar_base + 8u * (1 + 2 * RING + i); };
-  auto p_ready = [&](int n) { return bar_base + 8u * (1 + 2 * RING + NT + n); };  // tile i: 2i its first 64 keys, 2i + 1 the rest
-  auto o_done = [&](int i) { return bar_base + 8u * (1 + 2 * RING + 3 * NT + i); };
-  constexpr int N_BARS = 1 + 2 * RING + 4 * NT;
-  static_assert(N_BARS * 8 + 8 <= 256, "barrier area");
+  auto p_ready = [&](int i) { return bar_base + 8u * (1 + 2 * RING + NT + i); };
+  auto o_done = [&](int i) { return bar_base + 8u * (1 + 2 * RING + 2 * NT + i); };
+  auto top_ready = [&](int n) { return bar_base + 8u * (1 + 2 * RING + 3 * NT + n); };  // 4 * tile + quarter: both halves of 32 rows have their maximum there
+  constexpr int N_BARS = 1 + 2 * RING + 7 * NT;
+  static_assert(N_BARS * 8 + 8 <= 384, "barrier area");
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem_raw + C::BARS + N_BARS * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -87,14 +90,14 @@ rules_fwd_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     }
     for (int i = 0; i < NT; ++i) {
       mbar_init(s_full(i), 1);
-      mbar_init(p_ready(2 * i), 4);
-      mbar_init(p_ready(2 * i + 1), 4);
+      mbar_init(p_ready(i), 8);
       mbar_init(o_done(i), 1);
+      for (int n = 0; n < 4; ++n) mbar_init(top_ready(4 * i + n), 2);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 4 * NT + 1) {
+  if (warp == C::SOFTMAX + 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void*)tmem_slot)), "r"(C::TMEM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -104,19 +107,19 @@ rules_fwd_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const uint32_t tmem_base = *tmem_slot;
   const int end = last - first + 1;
 
-  // NT = 2: 384 threads x 168 registers at launch = 256 x 224 + 128 x 56
-  if (warp < 4 * NT) {
-    if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-    // ------------------------------------------------------------------ softmax and output, one thread per query row
-    const int i = warp >> 2, q = warp & 3;
+  if (warp < C::SOFTMAX) {
+    // ------------------------------------------------------------------ softmax and output: two threads a row, each with 64 of its keys
+    const int i = warp >> 3, half = warp >> 2 & 1, q = warp & 3;
     const int row = q * 32 + lane, qi = q0 + i * BLK + row;
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
-    const uint32_t tS = tmem_base + (uint32_t)(i * 128) + lane_base, tO = tmem_base + (uint32_t)(NT * 128 + i * D) + lane_base;
+    const uint32_t tS = tmem_base + (uint32_t)(i * 128 + half * 64) + lane_base, tO = tmem_base + (uint32_t)(NT * 128 + i * D) + lane_base;
+    float* exchange = reinterpret_cast<float*>(smem_raw + C::EXCHANGE) + i * 256 + row;
     const Score f = score_of(p, h);
     const bool cap = p.cap > 0.f;
-    // with neither a cap nor slopes the scale goes into the exponent's multiply-add
-    const bool folded = !cap && f.slope == 0.f && f.post > 0.f;
-    const float unit = folded ? f.post : 1.f;
+    // Without slopes a row's largest score is that of its largest product, if the scale is positive: the maximum is taken before the scores are
+    // made.  With neither a cap nor slopes the scale then goes into the exponent's multiply-add.
+    const bool direct = f.slope == 0.f && p.scale > 0.f, folded = direct && !cap;
+    const float unit = folded ? f.post : 1.f, post = folded ? 1.f : f.post;
     int lo, hi, own = 0;
     row_span(p, qi, prefix, lo, hi);
     if (qi >= p.Tq) hi = -1;
@@ -128,50 +131,51 @@ rules_fwd_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     for (int n = next(-1); n < end; n = next(n)) {
       const int fl = flags[n] >> (2 * i);
       if (!(fl & NEEDED)) continue;
-      const int k0 = (first + n) * BLK;
-      uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
-      if (!(fl & WHOLE)) {  // this row's 128 bits, while the score product runs
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          keep[c] = span_bits(lo, hi, k0 + c * 32);
-          if (p.seg_k != nullptr) {
-            const int k = k0 + c * 32 + lane;
-            keep[c] &= segment_bits(k < p.Tk ? p.seg_k[(long long)b * p.Tk + k] : -1, own);
-          }
+      const int k0 = (first + n) * BLK + half * 64;
+      const bool whole = (fl & WHOLE) != 0;
+      uint32_t keep0 = ~0u, keep1 = ~0u;
+      if (!whole) {  // this thread's 64 bits, while the score product runs
+        keep0 = span_bits(lo, hi, k0);
+        keep1 = span_bits(lo, hi, k0 + 32);
+        if (p.seg_k != nullptr) {
+          const int k = k0 + lane;
+          const int* seg = p.seg_k + (long long)b * p.Tk;
+          keep0 &= segment_bits(k < p.Tk ? seg[k] : -1, own);
+          keep1 &= segment_bits(k + 32 < p.Tk ? seg[k + 32] : -1, own);
         }
       }
       ok = mbar_wait(s_full(i), count & 1, abort_flag);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      float x[128];
+      // the maximum; scores are read from TMEM twice, so that only 32 of them are in registers at a time
+      float mx = -INFINITY;
+#pragma unroll 1
+      for (int c = 0; c < 2; ++c) {
+        float x[32];
+        tmem_ld32(tS + (uint32_t)(c * 32), reinterpret_cast<uint32_t*>(x));
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (!direct) scores32(x, cap, c_, post, f.slope, (float)(qi - k0 - c * 32));
+        if (!whole) {
+          const uint32_t keep = c == 0 ? keep0 : keep1;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(tS + (uint32_t)(c * 32), reinterpret_cast<uint32_t*>(x) + c * 32);
-      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-      if (cap) {
-        capped(x, f.pre);
-        const uint64_t post2 = both(f.post);
+          for (int e = 0; e < 32; ++e)
+            if (!(keep >> e & 1u)) x[e] = -INFINITY;
+        }
+        float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int e = 0; e < 128; e += 2) unpack_f32x2(mul_f32x2(pack_f32x2(x[e], x[e + 1]), post2), x[e], x[e + 1]);
-      } else if (!folded) {
+        for (int e = 0; e < 32; e += 8)
 #pragma unroll
-        for (int e = 0; e < 128; ++e) x[e] *= f.post;
+          for (int u = 0; u < 4; ++u) m4[u] = max3_nan(m4[u], x[e + u], x[e + 4 + u]);
+        mx = max_nan(max_nan(m4[0], m4[1]), max_nan(m4[2], m4[3]));
       }
-      if (f.slope != 0.f) {
-        const float from = (float)(qi - k0);
-#pragma unroll
-        for (int e = 0; e < 128; ++e) x[e] = fmaf(-f.slope, fabsf(from - (float)e), x[e]);
-      }
-      if (!(fl & WHOLE)) {
-#pragma unroll
-        for (int e = 0; e < 128; ++e)
-          if (!(keep[e >> 5] >> (e & 31) & 1u)) x[e] = -INFINITY;
-      }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int e = 0; e < 128; e += 8)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) mx[c] = max_nan(mx[c], max_nan(x[e + c], x[e + 4 + c]));
-      const float m_new = max_nan(m, max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * unit);
+      if (direct && mx != -INFINITY) mx = cap ? tanh_any(mx * f.pre) * f.post : mx * f.post;
+      float* slot = exchange + (count & 1) * (NT * 256);
+      slot[half * 128] = mx;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(top_ready(4 * i + q));
+      ok = mbar_wait(top_ready(4 * i + q), count & 1, abort_flag);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      const float m_new = max3_nan(m, mx, slot[(half ^ 1) * 128]);
       // a NaN or +inf among the scores makes the row NaN, whichever way its exponential goes
       l2[0] = add_f32x2(l2[0], pack_f32x2(m_new == -INFINITY ? 0.f : m_new - m_new, 0.f));
       const bool grow = m_new > m + RESCALE || (m == -INFINITY && m_new > m);
@@ -181,9 +185,9 @@ rules_fwd_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         const uint64_t a2 = both(alpha);
         l2[0] = fma_f32x2(l2[0], a2, 0);
         l2[1] = fma_f32x2(l2[1], a2, 0);
-        if (count > 0) {  // a full S also says that P V of the tile before has been added
+        if (count > 0) {  // a full S also says that P V of the tile before has been added; each of the two threads takes half of O
 #pragma unroll 1
-          for (int c = 0; c < D / 16; ++c) {
+          for (int c = half * (D / 32); c < (half + 1) * (D / 32); ++c) {
             uint32_t o[16];
             tmem_ld16(tO + (uint32_t)(c * 16), o);
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -194,13 +198,23 @@ rules_fwd_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         }
       }
       const uint64_t scale2 = both(unit), minus2 = both(m == -INFINITY ? 0.f : -m);
+#pragma unroll 1
+      for (int c = 0; c < 2; ++c) {
+        float x[32];
+        tmem_ld32(tS + (uint32_t)(c * 32), reinterpret_cast<uint32_t*>(x));
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        scores32(x, cap, c_, post, f.slope, (float)(qi - k0 - c * 32));
+        if (!whole) {
+          const uint32_t keep = c == 0 ? keep0 : keep1;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+          for (int e = 0; e < 32; ++e)
+            if (!(keep >> e & 1u)) x[e] = -INFINITY;
+        }
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           float x0, x1;
-          const uint64_t x2 = fma_f32x2(pack_f32x2(x[c * 32 + 2 * e], x[c * 32 + 2 * e + 1]), scale2, minus2);
+          const uint64_t x2 = fma_f32x2(pack_f32x2(x[2 * e], x[2 * e + 1]), scale2, minus2);
           if (e % 4 == 3 && !cap) {  // a quarter on the FMA pipe, which a cap keeps busy enough
             exp2_poly2(x2, x0, x1);
           } else {
@@ -212,80 +226,68 @@ rules_fwd_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           w[e] = pack_16<T>(x0, x1);
         }
         tmem_st16(tS + (uint32_t)(c * 16), w);
-        if (c & 1) {  // 64 keys are there: P V may start on them
-          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) mbar_arrive(p_ready(2 * i + (c >> 1)));
-        }
       }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_ready(i));
       ++count;
     }
     if (ok && count > 0) {
       ok = __all_sync(0xffffffffu, mbar_wait(o_done(i), 0, abort_flag));
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    } else if (ok && next(-1) < end) {
-      ok = __all_sync(0xffffffffu, mbar_wait(q_bar, 0, abort_flag));  // zeros are staged where Q may still be on its way, for the other tile's sake
     }
     if (ok) {
+      // both halves add the two sums in one order
       float la, lb, lc, ld;
       unpack_f32x2(l2[0], la, lb);
       unpack_f32x2(l2[1], lc, ld);
-      const float l = (la + lb) + (lc + ld);
+      float l = (la + lb) + (lc + ld);
+      if (count > 0) {  // the other half's sum: exchanged as the maxima were
+        float* slot = exchange + (count & 1) * (NT * 256);
+        slot[half * 128] = l;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(top_ready(4 * i + q));
+        ok = __all_sync(0xffffffffu, mbar_wait(top_ready(4 * i + q), count & 1, abort_flag));
+        l += slot[(half ^ 1) * 128];
+      }
       const bool blank = (m == -INFINITY && l == l) || qi >= p.Tq;
       const float inv_l = blank ? 0.f : 1.f / l;
-      // every product of this tile has completed: its Q is free, O is staged there; then what O's rounding lost, where it is asked for
+      // each of the two threads stores half of the row, and what its rounding lost where that is asked for
+      const long long at = (((long long)b * p.Tq + min(qi, p.Tq - 1)) * p.H + h) * p.D;
 #pragma unroll 1
-      for (int part = 0; part <= with_lo; ++part) {
-        if (part > 0) {
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-          __syncwarp();
+      for (int col = half * (D / 2); ok && col < (half + 1) * (D / 2); col += 32) {
+        float x[32];
+        if (count > 0) {
+          tmem_ld32(tO + (uint32_t)col, reinterpret_cast<uint32_t*>(x));
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         }
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          float o[32];
-          if (count > 0) {
-            tmem_ld32(tO + (uint32_t)(c * 32), reinterpret_cast<uint32_t*>(o));
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        for (int u = 0; u < 4; ++u) {
+          uint32_t w[4], lost[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float v0 = blank ? 0.f : x[u * 8 + 2 * e] * inv_l, v1 = blank ? 0.f : x[u * 8 + 2 * e + 1] * inv_l;
+            float r0, r1;
+            w[e] = pack_16<T>(v0, v1);
+            unpack_16<T>(w[e], r0, r1);
+            lost[e] = pack_16<T>(v0 - r0, v1 - r1);
           }
-          const uint32_t chunk = sQ + (uint32_t)(i * TILE + (c >> 1) * 16384) + (uint32_t)row * 128u;
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float v0 = blank ? 0.f : o[u * 8 + 2 * e] * inv_l, v1 = blank ? 0.f : o[u * 8 + 2 * e + 1] * inv_l;
-              w[e] = pack_16<T>(v0, v1);
-              if (part > 0) {
-                float r0, r1;
-                unpack_16<T>(w[e], r0, r1);
-                w[e] = pack_16<T>(v0 - r0, v1 - r1);
-              }
-            }
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(chunk + (((uint32_t)((c & 1) * 4 + u) ^ (uint32_t)(row & 7)) << 4)), "r"(w[0]), "r"(w[1]),
-                         "r"(w[2]), "r"(w[3]) : "memory");
+          if (qi < p.Tq && col + u * 8 < p.D) {
+            *reinterpret_cast<uint4*>(o + at + col + u * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (lo_out != nullptr) *reinterpret_cast<uint4*>(lo_out + at + col + u * 8) = make_uint4(lost[0], lost[1], lost[2], lost[3]);
           }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0 && q0 + i * BLK + q * 32 < p.Tq) {
-#pragma unroll
-          for (int c = 0; c < D / 64; ++c)
-            tma_store_4d(part == 0 ? &map_o : &map_lo, sQ + (uint32_t)(i * TILE + c * 16384) + (uint32_t)(q * 32) * 128u, c * 64, q0 + i * BLK + q * 32, h, b);
-          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
       }
-      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the writes land before the grid ends
-      if (lse != nullptr && qi < pitch) lse[((long long)b * p.H + h) * pitch + qi] = blank ? INFINITY : m + log2f(l);
+      if (lse != nullptr && half == 0 && qi < pitch) lse[((long long)b * p.H + h) * pitch + qi] = blank ? INFINITY : m + log2f(l);
     }
     if (!ok) {
       if (lane == 0 && err) atomicExch(err, 43);
       *abort_flag = 1;
     }
   } else {
-    if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     const int start = next(-1);
-    if (warp == 4 * NT) {
+    if (warp == C::SOFTMAX) {
       // ------------------------------------------------------------------ TMA producer
       if (elect_one() && start < end) {
         mbar_expect_tx(q_bar, NT * TILE);
@@ -324,7 +326,7 @@ rules_fwd_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
               if (mbar_try_wait(kv_full(n % RING), (n / RING) & 1)) break;
         }
       }
-    } else if (warp == 4 * NT + 1) {
+    } else {
       // ------------------------------------------------------------------ MMA issuer
       if (elect_one() && start < end) {
         constexpr uint32_t idesc_s = product_desc<T>(128, 128, false), idesc_o = product_desc<T>(128, D, true);
@@ -339,11 +341,11 @@ rules_fwd_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           }
           umma_commit(s_full(i));
         };
-        auto values = [&](int i, int s, int half, bool fresh) {  // 64 keys
-          const uint64_t bdesc = mn_desc(sKV + s * TILE + half * 8192, 16384);
+        auto values = [&](int i, int s, bool fresh) {
+          const uint64_t bdesc = mn_desc(sKV + s * TILE, 16384);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)  // 16 keys: 8 columns of packed pairs
-            umma_bf16_ts(tmem_O(i), tmem_S(i) + (uint32_t)(half * 32 + k * 8), bdesc + (uint64_t)((2048u >> 4) * k), idesc_o, (!fresh || half > 0 || k > 0) ? 1u : 0u);
+          for (int k = 0; k < 8; ++k)  // 16 keys: 8 columns of packed pairs, those of the second half behind that half's scores
+            umma_bf16_ts(tmem_O(i), tmem_S(i) + (uint32_t)((k >> 2) * 64 + (k & 3) * 8), bdesc + (uint64_t)((2048u >> 4) * k), idesc_o, (!fresh || k > 0) ? 1u : 0u);
         };
         int done[NT] = {0}, left[NT] = {0};
         for (int n = start; n < end; n = next(n))
@@ -367,14 +369,10 @@ rules_fwd_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           for (int i = 0; i < NT; ++i) {
             if (!ok) continue;
             if (needs(i, n)) {
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                if (ok) ok = mbar_wait(p_ready(2 * i + half), done[i] & 1, abort_flag);  // that half of P is in TMEM, S has been read, O rescaled
-                if (!ok) continue;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                values(i, nv % RING, half, done[i] == 0);
-              }
+              ok = mbar_wait(p_ready(i), done[i] & 1, abort_flag);  // P is in TMEM, S has been read, O rescaled
               if (!ok) continue;
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+              values(i, nv % RING, done[i] == 0);
               if (++done[i] == left[i]) umma_commit(o_done(i));
             }
             if (needs(i, then)) {
@@ -400,13 +398,13 @@ rules_fwd_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   __syncwarp();
-  if (warp == 4 * NT + 1) {
+  if (warp == C::SOFTMAX + 1) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(C::TMEM_COLS) : "memory");
   }
 }
 
 template <typename T, int D, int NT>
-int launch_fwd(const CUtensorMap* maps, const Rules& p, float* lse, int pitch, int with_lo, int* err, cudaStream_t stream) {
+int launch_fwd(const CUtensorMap* maps, const Rules& p, void* o, void* lo, float* lse, int pitch, int* err, cudaStream_t stream) {
   using C = FwdCfg<D, NT>;
   const int smem = C::SMEM + ((p.Tk + BLK - 1) / BLK + 15) / 16 * 16;
   static bool attr[KB_MAX_DEVICES] = {false};
@@ -415,7 +413,7 @@ int launch_fwd(const CUtensorMap* maps, const Rules& p, float* lse, int pitch, i
     return -3;
   }
   const long long grid = (long long)((p.Tq + 128 * NT - 1) / (128 * NT)) * p.H * p.B;
-  rules_fwd_sm100<T, D, NT><<<(unsigned)grid, C::THREADS_, smem, stream>>>(maps[0], maps[1], maps[2], maps[3], maps[4], p, lse, pitch, with_lo, err);
+  rules_fwd_sm100<T, D, NT><<<(unsigned)grid, C::THREADS_, smem, stream>>>(maps[0], maps[1], maps[2], p, make_cap(p.scale, p.cap), (T*)o, (T*)lo, lse, pitch, err);
   return 0;
 }
 
@@ -433,21 +431,18 @@ KB_API int kb200_attention_rules_fwd_sm100(const void* q, const void* k, const v
     return -2;
   }
   const Strides qs{strides[0], strides[1], strides[2]}, ks{strides[3], strides[4], strides[5]}, vs{strides[6], strides[7], strides[8]};
-  const Strides os{(long long)H * D, D, (long long)Tq * H * D};
   if (!rules_strides(qs, q, Tq, H, B) || !rules_strides(ks, k, Tk, Hkv, B) || !rules_strides(vs, v, Tk, Hkv, B) || (((uintptr_t)o | (uintptr_t)lo) & 15)) {
     kb200_set_error("attention_rules_fwd_sm100: strides and base pointers must be multiples of 16 bytes");
     return -2;
   }
   const bool half = dtype == 2;
-  CUtensorMap maps[5];
-  if (!rules_map(&maps[0], q, D, Tq, H, B, qs, 128, half) || !rules_map(&maps[1], k, D, Tk, Hkv, B, ks, 128, half) || !rules_map(&maps[2], v, D, Tk, Hkv, B, vs, 128, half) ||
-      !rules_map(&maps[3], o, D, Tq, H, B, os, 32, half) || !rules_map(&maps[4], lo != nullptr ? lo : o, D, Tq, H, B, os, 32, half)) {
+  CUtensorMap maps[3];
+  if (!rules_map(&maps[0], q, D, Tq, H, B, qs, 128, half) || !rules_map(&maps[1], k, D, Tk, Hkv, B, ks, 128, half) || !rules_map(&maps[2], v, D, Tk, Hkv, B, vs, 128, half)) {
     kb200_set_error("attention_rules_fwd_sm100: cuTensorMapEncodeTiled failed");
     return -3;
   }
-  const int with_lo = lo != nullptr ? 1 : 0;
   int rc;
-#define KB_CALL(DD, NT) (half ? launch_fwd<__half, DD, NT>(maps, p, lse, pitch, with_lo, err, stream) : launch_fwd<__nv_bfloat16, DD, NT>(maps, p, lse, pitch, with_lo, err, stream))
+#define KB_CALL(DD, NT) (half ? launch_fwd<__half, DD, NT>(maps, p, o, lo, lse, pitch, err, stream) : launch_fwd<__nv_bfloat16, DD, NT>(maps, p, o, lo, lse, pitch, err, stream))
   if (D <= 64) rc = Tq <= 128 ? KB_CALL(64, 1) : KB_CALL(64, 2);
   else rc = Tq <= 128 ? KB_CALL(128, 1) : KB_CALL(128, 2);
 #undef KB_CALL

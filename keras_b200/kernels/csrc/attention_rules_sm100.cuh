@@ -32,35 +32,72 @@ __device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
 }
 __device__ __forceinline__ uint64_t both(float a) { return pack_f32x2(a, a); }
 
-// tanh of two values of at most 1: x times a polynomial of degree 5 in x^2, fitted as tanh_small's (7e-7 of the value with its roundings, a
-// thousandth of what rounding the probabilities to 16 bits costs under a cap of 50).
-__device__ __forceinline__ uint64_t tanh_small2(uint64_t x) {
-  const uint64_t u = mul_f32x2(x, x);
-  uint64_t p = fma_f32x2(both(-0.0030670708511024714f), u, both(0.016743140295147896f));
-  p = fma_f32x2(p, u, both(-0.051605693995952606f));
-  p = fma_f32x2(p, u, both(0.13281434774398804f));
-  p = fma_f32x2(p, u, both(-0.3332904279232025f));
-  p = fma_f32x2(p, u, both(0.9999994039535522f));
-  return mul_f32x2(p, x);
+// The cap of a call as the kernels take it: tanh(s * pre) * post from polynomials in x^2 = (s * pre)^2 whose coefficients hold `post` already.
+struct Cap {
+  float pre, post, inv_post;
+  float near[4], far[6];
+};
+// tanh(x) / x for |x| <= 1/2 (degree 3 in x^2) and |x| <= 1 (degree 5), fitted as tanh_small's: 5.5e-7 and 5.9e-7 of the value, a thousandth of what rounding
+// the probabilities to 16 bits costs under a cap of 50.  As a rule scores stay below half of their cap, and tanh is six instructions on the
+// FMA pipe instead of an exponential and a reciprocal on the one that the softmax needs.
+static inline Cap make_cap(float scale, float cap) {
+  const float near[4] = {0.999999463558197f, -0.33326318860054016f, 0.13190299272537231f, -0.04440227895975113f};
+  const float far[6] = {0.9999994039535522f, -0.3332904279232025f, 0.13281434774398804f, -0.051605693995952606f, 0.016743140295147896f, -0.0030670708511024714f};
+  Cap c{};
+  if (cap > 0.f) {
+    c.pre = scale / cap;
+    c.post = cap * LOG2E;
+    c.inv_post = 1.f / c.post;
+    for (int i = 0; i < 4; ++i) c.near[i] = near[i] * c.post;
+    for (int i = 0; i < 6; ++i) c.far[i] = far[i] * c.post;
+  }
+  return c;
 }
 
-// x[e] := tanh(x[e] * pre), for a warp: on the FMA pipe as long as no lane has a value beyond 1.
-template <int N>
-__device__ __forceinline__ void capped(float (&x)[N], float pre) {
-  const uint64_t pre2 = both(pre);
+// 32 raw scores to tanh(s * pre) * post, for a warp, by the shortest form that all its lanes allow.
+__device__ __forceinline__ void capped(float (&x)[32], const Cap& c) {
+  const uint64_t pre2 = both(c.pre);
   float top = 0.f;
 #pragma unroll
-  for (int e = 0; e < N; e += 2) {
+  for (int e = 0; e < 32; e += 2) {
     unpack_f32x2(mul_f32x2(pack_f32x2(x[e], x[e + 1]), pre2), x[e], x[e + 1]);
-    top = fmaxf(top, fmaxf(fabsf(x[e]), fabsf(x[e + 1])));
+    top = fmaxf(fmaxf(top, fabsf(x[e])), fabsf(x[e + 1]));
   }
-  if (__any_sync(0xffffffffu, top > 1.f)) {
+  if (!__any_sync(0xffffffffu, top > 0.5f)) {
+    const uint64_t a0 = both(c.near[0]), a1 = both(c.near[1]), a2 = both(c.near[2]), a3 = both(c.near[3]);
 #pragma unroll
-    for (int e = 0; e < N; ++e) x[e] = tanh_any(x[e]);
+    for (int e = 0; e < 32; e += 2) {
+      const uint64_t v = pack_f32x2(x[e], x[e + 1]), u = mul_f32x2(v, v);
+      unpack_f32x2(mul_f32x2(fma_f32x2(fma_f32x2(fma_f32x2(a3, u, a2), u, a1), u, a0), v), x[e], x[e + 1]);
+    }
+  } else if (!__any_sync(0xffffffffu, top > 1.f)) {
+    const uint64_t a0 = both(c.far[0]), a1 = both(c.far[1]), a2 = both(c.far[2]), a3 = both(c.far[3]), a4 = both(c.far[4]), a5 = both(c.far[5]);
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      const uint64_t v = pack_f32x2(x[e], x[e + 1]), u = mul_f32x2(v, v);
+      unpack_f32x2(mul_f32x2(fma_f32x2(fma_f32x2(fma_f32x2(fma_f32x2(fma_f32x2(a5, u, a4), u, a3), u, a2), u, a1), u, a0), v), x[e], x[e + 1]);
+    }
   } else {
 #pragma unroll
-    for (int e = 0; e < N; e += 2) unpack_f32x2(tanh_small2(pack_f32x2(x[e], x[e + 1])), x[e], x[e + 1]);
+    for (int e = 0; e < 32; ++e) x[e] = tanh_any(x[e]) * c.post;
   }
+}
+// 32 raw scores to scores in log2; `from` - e is the distance of the pair.  A score that is not capped is multiplied with `post`.
+__device__ __forceinline__ void scores32(float (&x)[32], bool cap, const Cap& c, float post, float slope, float from) {
+  if (cap) capped(x, c);
+  else if (post != 1.f) {
+#pragma unroll
+    for (int e = 0; e < 32; ++e) x[e] *= post;
+  }
+  if (slope != 0.f) {
+#pragma unroll
+    for (int e = 0; e < 32; ++e) x[e] = fmaf(-slope, fabsf(from - (float)e), x[e]);
+  }
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 // Bits of the elements e of 32 with lo <= at + e <= hi.
