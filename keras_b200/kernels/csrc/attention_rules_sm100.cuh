@@ -36,6 +36,8 @@ __device__ __forceinline__ uint64_t both(float a) { return pack_f32x2(a, a); }
 struct Cap {
   float pre, post, inv_post;
   float near[4], far[6];
+  float near_raw[4];  // of x = s itself
+  bool folds;         // they are all well within the type
 };
 // tanh(x) / x for |x| <= 1/2 (degree 3 in x^2) and |x| <= 1 (degree 5), fitted as tanh_small's: 5.5e-7 and 5.9e-7 of the value, a thousandth of what rounding
 // the probabilities to 16 bits costs under a cap of 50.  As a rule scores stay below half of their cap, and tanh is six instructions on the
@@ -50,6 +52,10 @@ static inline Cap make_cap(float scale, float cap) {
     c.inv_post = 1.f / c.post;
     for (int i = 0; i < 4; ++i) c.near[i] = near[i] * c.post;
     for (int i = 0; i < 6; ++i) c.far[i] = far[i] * c.post;
+    const double a = fabs((double)c.pre);
+    c.folds = a > 1e-4 && a < 1e3 && cap > 1e-6f && cap < 1e6f;
+    if (c.folds)
+      for (int i = 0; i < 4; ++i) c.near_raw[i] = (float)(near[i] * (double)c.post * pow((double)c.pre, 2 * i + 1));
   }
   return c;
 }

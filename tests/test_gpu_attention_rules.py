@@ -35,20 +35,20 @@ def _definition(q, k, v, do, rules, scale=None):
 
 
 def _run(q, k, v, do, rules):
-    """Results and gradients, and that kernels made them."""
+    """Results and gradients, and that kernels made them; the result without gradients, whose rounding of the probabilities may differ, last."""
     before = kops.launch_count()
     leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
     out = keras.ops.dot_product_attention(*leaves, **rules)
     grads = torch.autograd.grad(out, leaves, do)
     assert kops.launch_count() - before >= 3
     with torch.no_grad():
-        assert torch.equal(keras.ops.dot_product_attention(q, k, v, **rules), out.detach())
-    return (out.detach(), *grads)
+        alone = keras.ops.dot_product_attention(q, k, v, **rules)
+    return (out.detach(), *grads, alone)
 
 
 def _check(q, k, v, do, rules):
     found = _definition(q, k, v, do, rules)
-    for name, got in zip(("out", "dq", "dk", "dv"), _run(q, k, v, do, rules)):
+    for name, got in zip(("out", "dq", "dk", "dv", "out"), _run(q, k, v, do, rules)):
         assert got.dtype == q.dtype
         definition.check(name, got, found)
 
