@@ -37,7 +37,10 @@ def launcher(name, arguments):
 
 def strides(*tensors):
     """Strides of time, heads and batch of each, as the C entries take them; a dimension of one element may carry any."""
-    flat = [0 if t.shape[i] == 1 else t.stride(i) for t in tensors for i in (1, 2, 0)]
+    flat = []
+    for t in tensors:
+        (b, n, h, _), (sb, sn, sh, _) = t.shape, t.stride()
+        flat += (0 if n == 1 else sn, 0 if h == 1 else sh, 0 if b == 1 else sb)
     return (ctypes.c_longlong * len(flat))(*flat)
 
 
@@ -46,22 +49,69 @@ def unit(t):
     return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
 
 
+class Plan:
+    """What a call's types, sizes and strides settle: worked out once for each and kept, as a step calls the same layers again and again."""
+
+    __slots__ = ("fits", "unit", "tensor", "tiled", "grad_strides", "code", "sizes", "out", "lse", "pitch", "strides")
+
+    def __init__(self, q, k, v):
+        same = (q.dtype in _CODES and k.dtype == q.dtype and v.dtype == q.dtype and k.shape == v.shape and k.shape[0] == q.shape[0] and k.shape[-1] == q.shape[-1]
+                and 0 not in q.shape and 0 not in k.shape and q.shape[2] % k.shape[2] == 0 and q.shape[-1] <= MAX_HEAD)
+        B, T, H, D = q.shape
+        S, K = k.shape[1:3]
+        self.fits = same and ((T + 31) // 32) * H * B < 1 << 31 and ((S + 31) // 32) * H * B < 1 << 31
+        if not self.fits:
+            return
+        self.unit = D == 1 or q.stride(3) == k.stride(3) == v.stride(3) == 1
+        self.code = _CODES[q.dtype]
+        # whether the tensor-core kernels take heads of this size and type; layouts they do not read are copied for them
+        self.tensor = q.dtype != torch.float32 and D <= 128 and D % 8 == 0 and T <= MAX_LENGTH and S <= MAX_LENGTH
+        # strides that tile copies can read: multiples of 16 bytes, none of them zero
+        self.tiled = all(n == 1 or (s > 0 and s % 8 == 0) for t in (q, k, v) for n, s in zip(t.shape[:3], t.stride()))
+        self.sizes = (B, H, K, T, S, D)
+        self.out, self.pitch = (B, T, H, D), (T + 127) // 128 * 128
+        self.lse = (B, H, self.pitch)
+        self.strides = strides(q, k, v)
+        o = (0 if T == 1 else H * D, 0 if H == 1 else D, 0 if B == 1 else T * H * D)
+        self.grad_strides = (ctypes.c_longlong * 12)(*self.strides, *o)  # with a contiguous gradient of the result
+
+
+_PLANS = {}
+
+
+def plan_of(q, k, v):
+    key = (q.dtype, k.dtype, v.dtype, q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride())
+    plan = _PLANS.get(key)
+    if plan is None:
+        if len(_PLANS) >= 1024:  # sizes that change with every call
+            _PLANS.clear()
+        plan = _PLANS[key] = Plan(q, k, v)
+    return plan
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+_RANGES_ARGS = [_V, _V, _I, _I, _V]
+
+
 def _ranges(seg):
-    out = torch.empty((seg.shape[0], (seg.shape[1] + 127) // 128, 4), dtype=torch.int32, device=seg.device)
-    code = launcher("kb200_segment_ranges", [_V, _V, _I, _I, _V])(seg.data_ptr(), out.data_ptr(), seg.shape[0], seg.shape[1], kops._stream())
+    B, T = seg.shape
+    out = torch.empty((B, (T + 127) // 128, 4), dtype=torch.int32, device=seg.device)
+    code = launcher("kb200_segment_ranges", _RANGES_ARGS)(seg.data_ptr(), out.data_ptr(), B, T, kops._stream())
     kops._check(code, "segment_ranges")
     return out
 
 
 def _tail(rules, ranges):
     """The arguments that say the rules, the stream included."""
-    seg = rules.segments or (None, None)
-    return (rules.scale, rules.cap or 0.0, _ptr(rules.slopes), 1 if rules.causal else 0, min(rules.window or 0, 1 << 30), _ptr(rules.prefix), _ptr(seg[0]), _ptr(seg[1]),
-            _ptr(ranges[0]), _ptr(ranges[1]), kops._stream())
+    if rules.segments is None:
+        seg_q = seg_k = range_q = range_k = None
+    else:
+        seg_q, seg_k, range_q, range_k = (t.data_ptr() for t in (*rules.segments, *ranges))
+    return (rules.scale, rules.cap or 0.0, _ptr(rules.slopes), 1 if rules.causal else 0, min(rules.window or 0, 1 << 30), _ptr(rules.prefix), seg_q, seg_k, range_q, range_k,
+            kops._stream())
 
 
 def segment_ranges(rules):
@@ -72,11 +122,6 @@ def segment_ranges(rules):
     return first, first if keys is rows else _ranges(keys)
 
 
-def tensor_cores(q, k, v):
-    """Whether the tensor-core kernels take heads of this size and type; layouts they do not read are copied for them."""
-    return q.dtype != torch.float32 and q.shape[-1] <= 128 and q.shape[-1] % 8 == 0 and q.shape[1] <= MAX_LENGTH and k.shape[1] <= MAX_LENGTH
-
-
 def _tiles(t):
     """A tensor that tile copies can read: base and strides multiples of 16 bytes, none of them zero."""
     if t.data_ptr() % 16 == 0 and all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:3], t.stride())):
@@ -84,90 +129,100 @@ def _tiles(t):
     return kops.aligned(t)
 
 
-def _pitch(T):
-    return (T + 127) // 128 * 128
+_FWD_SM100 = [_V] * 6 + [_I, _V] + [_I] * 7 + [_V] + _RULES
+_FWD = [_V] * 5 + [_I, _V] + [_I] * 7 + _RULES
+_GRADS = [_V] * 9 + [_I] + [_V] * 3 + [_I] * 7 + [_V] + _RULES
 
 
-def forward(q, k, v, rules, ranges, training):
+def forward(q, k, v, rules, ranges, training, plan=None):
     """``(out [B, Tq, H, D], lse [B, H, pitch] float32, lo)``; the sums of a row are kept as log2, ``lo`` is what rounding the result lost, both for the
     gradients alone."""
-    B, Tq, H, D = q.shape
-    out = torch.empty((B, Tq, H, D), dtype=q.dtype, device=q.device)
-    pitch = _pitch(Tq)
-    lse = torch.empty((B, H, pitch), dtype=torch.float32, device=q.device) if training else None
-    sizes = (_CODES[q.dtype], B, H, k.shape[2], Tq, k.shape[1], D)
-    if tensor_cores(q, k, v):
-        q, k, v = _tiles(q), _tiles(k), _tiles(v)
-        lo = torch.empty_like(out) if training else None
-        code = launcher("kb200_attention_rules_fwd_sm100", [_V] * 6 + [_I, _V] + [_I] * 7 + [_V] + _RULES)(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lo), _ptr(lse), pitch, strides(q, k, v), *sizes, _err_flag(q.device).data_ptr(),
-            *_tail(rules, ranges))
+    plan = plan or plan_of(q, k, v)
+    out = q.new_empty(plan.out)
+    lse = q.new_empty(plan.lse, dtype=torch.float32) if training else None
+    if plan.tensor:
+        a, b, c = q.data_ptr(), k.data_ptr(), v.data_ptr()
+        layout = plan.strides
+        if not plan.tiled or (a | b | c) % 16:
+            q, k, v = _tiles(q), _tiles(k), _tiles(v)
+            a, b, c = q.data_ptr(), k.data_ptr(), v.data_ptr()
+            layout = strides(q, k, v)
+        lo = q.new_empty(plan.out) if training else None
+        code = launcher("kb200_attention_rules_fwd_sm100", _FWD_SM100)(
+            a, b, c, out.data_ptr(), _ptr(lo), _ptr(lse), plan.pitch, layout, plan.code, *plan.sizes, _err_flag(q.device).data_ptr(), *_tail(rules, ranges))
         kops._check(code, "attention_rules_fwd_sm100")
         return out, lse, lo
-    code = launcher("kb200_attention_rules_fwd", [_V] * 5 + [_I, _V] + [_I] * 7 + _RULES)(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), pitch, strides(q, k, v), *sizes, *_tail(rules, ranges))
+    code = launcher("kb200_attention_rules_fwd", _FWD)(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse), plan.pitch, plan.strides, plan.code, *plan.sizes, *_tail(rules, ranges))
     kops._check(code, "attention_rules_fwd")
     return out, lse, None
 
 
-def backward(q, k, v, out, lo, lse, grad_out, rules, ranges, want_q, want_kv):
-    B, Tq, H, D = q.shape
-    Tk, Hkv, pitch = k.shape[1], k.shape[2], lse.shape[2]
-    tensor = tensor_cores(q, k, v)
-    grad_out = unit(grad_out)
-    if tensor:
-        q, k, v, grad_out = _tiles(q), _tiles(k), _tiles(v), _tiles(grad_out)
+def backward(q, k, v, out, lo, lse, grad_out, rules, ranges, want_q, want_kv, plan=None):
+    plan = plan or plan_of(q, k, v)
+    tensor = plan.tensor
+    a, b, c, d = q.data_ptr(), k.data_ptr(), v.data_ptr(), grad_out.data_ptr()
+    layout = plan.grad_strides
+    if not grad_out.is_contiguous() or (tensor and (not plan.tiled or (a | b | c | d) % 16)):
+        grad_out = unit(grad_out)
+        if tensor:
+            q, k, v, grad_out = _tiles(q), _tiles(k), _tiles(v), _tiles(grad_out)
+        a, b, c, d = q.data_ptr(), k.data_ptr(), v.data_ptr(), grad_out.data_ptr()
+        layout = strides(q, k, v, grad_out)
     delta = torch.empty_like(lse)
-    code = launcher("kb200_attention_rules_delta", [_V] * 5 + [_I] * 6 + [_V])(
-        out.data_ptr(), _ptr(lo), grad_out.data_ptr(), strides(grad_out), delta.data_ptr(), pitch, _CODES[q.dtype], B, H, Tq, D, kops._stream())
-    kops._check(code, "attention_rules_delta")
-    dq = torch.empty((B, Tq, H, D), dtype=q.dtype, device=q.device) if want_q else None
-    dk, dv = (torch.empty((B, Tk, Hkv, D), dtype=q.dtype, device=q.device) if want_kv else None for _ in range(2))
-    name = "kb200_attention_rules_bwd_sm100" if tensor else "kb200_attention_rules_bwd"
-    code = launcher(name, [_V] * 7 + [_I] + [_V] * 3 + [_I] * 7 + ([_V] if tensor else []) + _RULES)(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), grad_out.data_ptr(), strides(q, k, v, grad_out), lse.data_ptr(), delta.data_ptr(), pitch, _ptr(dq), _ptr(dk), _ptr(dv),
-        _CODES[q.dtype], B, H, Hkv, Tq, Tk, D, *((_err_flag(q.device).data_ptr(),) if tensor else ()), *_tail(rules, ranges))
+    dq = q.new_empty(plan.out) if want_q else None
+    dk = dv = None
+    if want_kv:
+        B, _, K, _, S, D = plan.sizes
+        dk, dv = q.new_empty((B, S, K, D)), q.new_empty((B, S, K, D))
+    # the sums of out * grad_out, then the gradients
+    name = "kb200_attention_rules_grads_sm100" if tensor else "kb200_attention_rules_grads"
+    code = launcher(name, _GRADS)(
+        a, b, c, out.data_ptr(), _ptr(lo), d, layout, lse.data_ptr(), delta.data_ptr(), plan.pitch,
+        _ptr(dq), _ptr(dk), _ptr(dv), plan.code, *plan.sizes, _err_flag(q.device).data_ptr(), *_tail(rules, ranges))
     kops._check(code, name[6:])
+    kops.add_launches(1)  # two launchers in one call
     return dq, dk, dv
 
 
 class RuleAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, slopes, prefix, rows, keys, rules, plain):
+    def forward(ctx, q, k, v, slopes, prefix, rows, keys, rules, plain, plan):
         ranges = segment_ranges(rules)
-        out, lse, lo = forward(q, k, v, rules, ranges, training=True)
+        out, lse, lo = forward(q, k, v, rules, ranges, True, plan)
         # the rules' tensors are saved too: one that is written to before the backward pass is an error, as for any operand
         ctx.save_for_backward(q, k, v, out, lo, lse, *ranges, slopes, prefix, rows, keys)
-        ctx.rules, ctx.plain = rules._replace(slopes=None, prefix=None, segments=None), plain
+        ctx.rules, ctx.plain, ctx.plan = Rules(rules.scale, rules.cap, None, rules.causal, rules.window, None, None), plain, plan
         return out
 
     @staticmethod
     def backward(ctx, grad_out):
         q, k, v, out, lo, lse, range_q, range_k, slopes, prefix, rows, keys = ctx.saved_tensors
-        rules = ctx.rules._replace(slopes=slopes, prefix=prefix, segments=None if rows is None else (rows, keys))
+        r = ctx.rules
+        rules = Rules(r.scale, r.cap, slopes, r.causal, r.window, prefix, None if rows is None else (rows, keys))
         need = ctx.needs_input_grad
         if torch.is_grad_enabled():  # the gradient is differentiated in its turn
             wanted = [t for t, n in zip((q, k, v), need) if n]
             given = iter(torch.autograd.grad(ctx.plain(q, k, v, rules), wanted, grad_out, create_graph=True))
             grads = [next(given) if n else None for n in need[:3]]
         else:
-            dq, dk, dv = backward(q, k, v, out, lo, lse, grad_out, rules, (range_q, range_k), need[0], need[1] or need[2])
+            dq, dk, dv = backward(q, k, v, out, lo, lse, grad_out, rules, (range_q, range_k), need[0], need[1] or need[2], ctx.plan)
             grads = [dq, dk if need[1] else None, dv if need[2] else None]
-        return (*grads, None, None, None, None, None, None)
+        return (*grads, None, None, None, None, None, None, None)
 
 
 def attention(q, k, v, rules, plain):
     """Attention on this package's kernels, or ``None`` when the call does not fit them.  ``plain(q, k, v, rules)``: the form that second
     derivatives go through."""
-    if (q.dtype not in _CODES or k.dtype != q.dtype or v.dtype != q.dtype or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[-1] != q.shape[-1]
-            or not q.device == k.device == v.device or 0 in q.shape or 0 in k.shape or q.shape[2] % k.shape[2] or q.shape[-1] > MAX_HEAD):
+    if not q.device == k.device == v.device or torch.is_autocast_enabled("cuda"):
         return None
-    if torch.is_autocast_enabled("cuda"):
+    plan = plan_of(q, k, v)
+    if not plan.fits:
         return None
-    if ((q.shape[1] + 31) // 32) * q.shape[2] * q.shape[0] >= 1 << 31 or ((k.shape[1] + 31) // 32) * q.shape[2] * q.shape[0] >= 1 << 31:
-        return None
-    q, k, v = unit(q), unit(k), unit(v)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if not plan.unit:
+        q, k, v = unit(q), unit(k), unit(v)
+        plan = plan_of(q, k, v)
+    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         rows, keys = rules.segments or (None, None)
-        return RuleAttention.apply(q, k, v, rules.slopes, rules.prefix, rows, keys, rules, plain)
-    return forward(q, k, v, rules, segment_ranges(rules), training=False)[0]
+        return RuleAttention.apply(q, k, v, rules.slopes, rules.prefix, rows, keys, rules, plain, plan)
+    return forward(q, k, v, rules, segment_ranges(rules), False, plan)[0]

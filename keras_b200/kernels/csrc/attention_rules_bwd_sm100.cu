@@ -613,3 +613,17 @@ KB_API int kb200_attention_rules_bwd_sm100(const void* q, const void* k, const v
   KB_CHECK_LAUNCH("attention_rules_bwd_sm100");
   return 0;
 }
+
+KB_API int kb200_attention_rules_delta(const void* o, const void* lo, const void* grad_out, const long long* strides, float* delta, int pitch, int dtype, int B, int H, int Tq, int D,
+                                       cudaStream_t stream);
+
+// All of a gradient in one call: delta, from o, lo (may be null) and grad_out, then the above.
+KB_API int kb200_attention_rules_grads_sm100(const void* q, const void* k, const void* v, const void* o, const void* lo, const void* grad_out, const long long* strides,
+                                             const float* lse, float* delta, int pitch, void* dq, void* dk, void* dv, int dtype, int B, int H, int Hkv, int Tq, int Tk, int D, int* err,
+                                             float scale, float cap, const float* slopes, int causal, int window, const int* prefix, const int* seg_q, const int* seg_k,
+                                             const void* range_q, const void* range_k, cudaStream_t stream) {
+  const int rc = kb200_attention_rules_delta(o, lo, grad_out, strides + 9, delta, pitch, dtype, B, H, Tq, D, stream);
+  return rc != 0 ? rc
+                 : kb200_attention_rules_bwd_sm100(q, k, v, grad_out, strides, lse, delta, pitch, dq, dk, dv, dtype, B, H, Hkv, Tq, Tk, D, err, scale, cap, slopes, causal, window, prefix,
+                                                   seg_q, seg_k, range_q, range_k, stream);
+}

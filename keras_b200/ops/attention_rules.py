@@ -163,8 +163,11 @@ def capped(q, k, v, scale, is_causal, cap):
 
 
 # ------------------------------------------------------------------------------------------------ the paged cache
+_CACHE = {"key", "value", "pages", "lengths"}
+
+
 def _cache_parts(cache, q, k, v):
-    if not isinstance(cache, Mapping) or set(cache) != {"key", "value", "pages", "lengths"}:
+    if not isinstance(cache, Mapping) or cache.keys() != _CACHE:
         _refuse("`cache` has to be a dict of `key`, `value`, `pages` and `lengths`.")
     pool_k, pool_v, pages, lengths = (cache[n] for n in ("key", "value", "pages", "lengths"))
     for name, t in cache.items():

@@ -687,6 +687,9 @@ def _whole_rows(t, T, S):
     return t.expand(torch.broadcast_shapes(t.shape, (T, S)))
 
 
+_ATTENTION_FLOATS = frozenset((torch.float32, torch.bfloat16, torch.float16))
+
+
 @op("nn")
 def dot_product_attention(query, key, value, bias=None, mask=None, scale=None, is_causal=False, flash_attention=None, attn_logits_soft_cap=None,
                           distance_slopes=None, sliding_window=None, segment_ids=None, prefix_lengths=None, cache=None):
@@ -720,8 +723,10 @@ def dot_product_attention(query, key, value, bias=None, mask=None, scale=None, i
     q, k, v = _t(query), _t(key), _t(value)
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
         raise ValueError(f"`dot_product_attention` only supports 4D inputs. Received: query.shape={tuple(q.shape)}, key.shape={tuple(k.shape)}, value.shape={tuple(v.shape)}.")
-    d = to_torch_dtype(result_type(q.dtype, k.dtype, v.dtype))
-    q, k, v = q.to(d), k.to(d), v.to(d)
+    d = q.dtype
+    if not (d == k.dtype == v.dtype and d in _ATTENTION_FLOATS):  # of one such type they stay as they are
+        d = to_torch_dtype(result_type(q.dtype, k.dtype, v.dtype))
+        q, k, v = q.to(d), k.to(d), v.to(d)
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     if cache is not None:
