@@ -52,7 +52,7 @@ def unit(t):
 class Plan:
     """What a call's types, sizes and strides settle: worked out once for each and kept, as a step calls the same layers again and again."""
 
-    __slots__ = ("fits", "unit", "tensor", "tiled", "grad_strides", "code", "sizes", "out", "lse", "pitch", "strides")
+    __slots__ = ("fits", "unit", "tensor", "tiled", "grad_strides", "code", "sizes", "out", "lse", "pitch", "strides", "_work")
 
     def __init__(self, q, k, v):
         same = (q.dtype in _CODES and k.dtype == q.dtype and v.dtype == q.dtype and k.shape == v.shape and k.shape[0] == q.shape[0] and k.shape[-1] == q.shape[-1]
@@ -63,7 +63,7 @@ class Plan:
         if not self.fits:
             return
         self.unit = D == 1 or q.stride(3) == k.stride(3) == v.stride(3) == 1
-        self.code = _CODES[q.dtype]
+        self.code, self._work = _CODES[q.dtype], None
         # whether the tensor-core kernels take heads of this size and type; layouts they do not read are copied for them
         self.tensor = q.dtype != torch.float32 and D <= 128 and D % 8 == 0 and T <= MAX_LENGTH and S <= MAX_LENGTH
         # strides that tile copies can read: multiples of 16 bytes, none of them zero
@@ -74,6 +74,15 @@ class Plan:
         self.strides = strides(q, k, v)
         o = (0 if T == 1 else H * D, 0 if H == 1 else D, 0 if B == 1 else T * H * D)
         self.grad_strides = (ctypes.c_longlong * 12)(*self.strides, *o)  # with a contiguous gradient of the result
+
+
+    def work(self):
+        """Floats of workspace of the gradients of key and value."""
+        if self._work is None:
+            fn = launcher("kb200_attention_rules_bwd_work" if self.tensor else "kb200_attention_rules_bwd_work_plain", [_I] * 6)
+            fn.restype = ctypes.c_longlong
+            self._work = fn(*self.sizes)
+        return self._work
 
 
 _PLANS = {}
@@ -131,7 +140,7 @@ def _tiles(t):
 
 _FWD_SM100 = [_V] * 6 + [_I, _V] + [_I] * 7 + [_V] + _RULES
 _FWD = [_V] * 5 + [_I, _V] + [_I] * 7 + _RULES
-_GRADS = [_V] * 9 + [_I] + [_V] * 3 + [_I] * 7 + [_V] + _RULES
+_GRADS = [_V] * 9 + [_I] + [_V] * 3 + [_I] * 7 + [_V, _V, ctypes.c_longlong] + _RULES
 
 
 def forward(q, k, v, rules, ranges, training, plan=None):
@@ -171,15 +180,19 @@ def backward(q, k, v, out, lo, lse, grad_out, rules, ranges, want_q, want_kv, pl
         layout = strides(q, k, v, grad_out)
     delta = torch.empty_like(lse)
     dq = q.new_empty(plan.out) if want_q else None
-    dk = dv = None
+    dk = dv = work = None
+    floats = 0
     if want_kv:
         B, _, K, _, S, D = plan.sizes
         dk, dv = q.new_empty((B, S, K, D)), q.new_empty((B, S, K, D))
+        floats = plan.work()
+        if floats:  # from the caching allocator, for this call and stream alone: a recorded graph has its own
+            work = q.new_empty(floats, dtype=torch.float32)
     # the sums of out * grad_out, then the gradients
     name = "kb200_attention_rules_grads_sm100" if tensor else "kb200_attention_rules_grads"
     code = launcher(name, _GRADS)(
         a, b, c, out.data_ptr(), _ptr(lo), d, layout, lse.data_ptr(), delta.data_ptr(), plan.pitch,
-        _ptr(dq), _ptr(dk), _ptr(dv), plan.code, *plan.sizes, _err_flag(q.device).data_ptr(), *_tail(rules, ranges))
+        _ptr(dq), _ptr(dk), _ptr(dv), plan.code, *plan.sizes, _err_flag(q.device).data_ptr(), _ptr(work), floats, *_tail(rules, ranges))
     kops._check(code, name[6:])
     kops.add_launches(1)  # two launchers in one call
     return dq, dk, dv

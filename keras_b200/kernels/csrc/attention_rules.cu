@@ -313,16 +313,35 @@ __device__ __forceinline__ void rule_gradient(const Rules& r, const Score& f, bo
   ds = seen ? p * (dp - delta) * through : 0.f;
 }
 
+// A key tile's walk over the query heads of its group and their row tiles, and how many blocks share it.
+struct Parts {
+  int count;    // 1: gradients are stored as they are
+  float* sums;  // [dk, dv][count][B, Tk, Hkv, D]
+};
+// dk and dv from the sums of their parts, in order.
+template <typename T>
+__global__ void __launch_bounds__(256) join_parts_kernel(const float* sums, T* dk, T* dv, int parts, long long n, float scale) {
+  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (at >= 2 * n) return;
+  const bool second = at >= n;
+  const long long e = second ? at - n : at;
+  const float* from = sums + (second ? (long long)parts * n : 0) + e;
+  float x = from[0];
+  for (int i = 1; i < parts; ++i) x += from[i * n];
+  (second ? dv : dk)[e] = from_f32<T>(x * (second ? 1.f : scale));
+}
+
 template <typename T, int DP, int BT>
 __global__ void __launch_bounds__(256) rules_dkv_kernel(const Rules r, const T* q, Strides qs, const T* k, Strides ks, const T* v, Strides vs, const Gradients g, T* dk, T* dv,
-                                                        int vec) {
+                                                        const Parts parts, int vec) {
   using C = Tile<T, DP, BT>;
   constexpr int M = BT / 16;
   extern __shared__ __align__(16) float sm[];
   float *sK = sm, *sV = sK + C::FLOATS, *sQ = sV + C::FLOATS, *sG = sQ + C::FLOATS, *sP = sG + C::FLOATS, *sD = sP + BT * C::SP, *sL = sD + BT * C::SP, *sE = sL + BT;
   int* sS = reinterpret_cast<int*>(sE + BT);
-  const int heads = r.Hkv * r.B, k0 = (int)(blockIdx.x / heads) * BT;  // a causal mask gives the first keys the most rows
-  const int hkv = (int)(blockIdx.x % heads) % r.Hkv, b = (int)(blockIdx.x % heads) / r.Hkv, group = r.H / r.Hkv;
+  const int unit = (int)(blockIdx.x / parts.count), part = (int)(blockIdx.x % parts.count);
+  const int heads = r.Hkv * r.B, k0 = unit / heads * BT;  // a causal mask gives the first keys the most rows
+  const int hkv = unit % heads % r.Hkv, b = unit % heads / r.Hkv, group = r.H / r.Hkv;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   load_tile<T, DP, BT>(sK, k + b * ks.b + hkv * ks.h, ks.t, k0, r.Tk, r.D, vec & 2);
   load_tile<T, DP, BT>(sV, v + b * vs.b + hkv * vs.h, vs.t, k0, r.Tk, r.D, vec & 4);
@@ -337,10 +356,17 @@ __global__ void __launch_bounds__(256) rules_dkv_kernel(const Rules r, const T* 
   }
   int first, last;
   rows_of_keys(r, k0, min(k0 + BT, r.Tk) - 1, prefix, first, last);
-  for (int h = hkv * group; h < (hkv + 1) * group; ++h) {
+  // the walk over the group's heads and their tiles of rows, or a part of it
+  const int tiles = last >= first ? last / BT - first / BT + 1 : 0;
+  const long long total = (long long)tiles * group, per = (total + parts.count - 1) / parts.count, begin = part * per, end = begin + per < total ? begin + per : total;
+  for (int h = hkv * group + (tiles > 0 ? (int)(begin / tiles) : 0); h < (hkv + 1) * group; ++h) {
+    const long long at = (long long)(h - hkv * group) * tiles;  // of the head's first tile
+    if (at >= end) break;
     const Score f = score_of(r, h);
     const float *lse = g.lse + ((long long)b * r.H + h) * g.pitch, *delta = g.delta + ((long long)b * r.H + h) * g.pitch;
-    for (int q0 = first / BT * BT; q0 <= last; q0 += BT) {
+    const int from = (int)(begin > at ? begin - at : 0), to = (int)(end - at < tiles ? end - at : tiles);
+    for (int n = from; n < to; ++n) {
+      const int q0 = (first / BT + n) * BT;
       if (!segments_meet(r, b, q0, k0)) continue;
       __syncthreads();
       load_tile<T, DP, BT>(sQ, q + b * qs.b + h * qs.h, qs.t, q0, r.Tq, r.D, vec & 1);
@@ -383,6 +409,12 @@ __global__ void __launch_bounds__(256) rules_dkv_kernel(const Rules r, const T* 
     scale[i] = r.scale;
   }
   const long long base = ((long long)b * r.Tk * r.Hkv + hkv) * r.D, pitch = (long long)r.Hkv * r.D;
+  if (parts.count > 1) {
+    const long long size = (long long)r.B * r.Tk * r.Hkv * r.D;
+    store_rows<float, DP, M>(parts.sums + part * size + base, pitch, ak, one, k0, r.Tk, r.D, ty, tx);
+    store_rows<float, DP, M>(parts.sums + (parts.count + part) * size + base, pitch, av, one, k0, r.Tk, r.D, ty, tx);
+    return;
+  }
   store_rows<T, DP, M>(dk + base, pitch, ak, scale, k0, r.Tk, r.D, ty, tx);
   store_rows<T, DP, M>(dv + base, pitch, av, one, k0, r.Tk, r.D, ty, tx);
 }
@@ -484,7 +516,7 @@ int rules_fwd(const Rules& r, const void* q, Strides qs, const void* k, Strides 
 }
 template <typename T, int DP, int BT>
 int rules_bwd(const Rules& r, const void* q, Strides qs, const void* k, Strides ks, const void* v, Strides vs, const Gradients& g, void* dq, void* dk, void* dv,
-              cudaStream_t stream) {
+              const Parts& parts, cudaStream_t stream) {
   using C = Tile<T, DP, BT>;
   constexpr int SMEM_KV = (4 * C::FLOATS + 2 * BT * C::SP + 3 * BT) * 4, SMEM_Q = (4 * C::FLOATS + BT * C::SP) * 4;
   static bool attr[2][KB_MAX_DEVICES] = {{false}};
@@ -494,8 +526,12 @@ int rules_bwd(const Rules& r, const void* q, Strides qs, const void* k, Strides 
   }
   const int vec = (vectors<T>(q, qs, r.D) ? 1 : 0) | (vectors<T>(k, ks, r.D) ? 2 : 0) | (vectors<T>(v, vs, r.D) ? 4 : 0) | (vectors<T>(g.grad_out, g.go, r.D) ? 8 : 0);
   if (dk != nullptr)
-    rules_dkv_kernel<T, DP, BT><<<(unsigned)((long long)((r.Tk + BT - 1) / BT) * r.Hkv * r.B), 256, SMEM_KV, stream>>>(r, (const T*)q, qs, (const T*)k, ks, (const T*)v, vs, g,
-                                                                                                                   (T*)dk, (T*)dv, vec);
+    rules_dkv_kernel<T, DP, BT><<<(unsigned)((long long)((r.Tk + BT - 1) / BT) * r.Hkv * r.B * parts.count), 256, SMEM_KV, stream>>>(r, (const T*)q, qs, (const T*)k, ks, (const T*)v, vs, g,
+                                                                                                                   (T*)dk, (T*)dv, parts, vec);
+  if (dk != nullptr && parts.count > 1) {
+    const long long n = (long long)r.B * r.Tk * r.Hkv * r.D;
+    join_parts_kernel<T><<<(unsigned)((2 * n + 255) / 256), 256, 0, stream>>>(parts.sums, (T*)dk, (T*)dv, parts.count, n, r.scale);
+  }
   if (dq != nullptr)
     rules_dq_kernel<T, DP, BT><<<(unsigned)((long long)((r.Tq + BT - 1) / BT) * r.H * r.B), 256, SMEM_Q, stream>>>(r, (const T*)q, qs, (const T*)k, ks, (const T*)v, vs, g, (T*)dq, vec);
   return 0;
@@ -579,16 +615,36 @@ KB_API int kb200_attention_rules_delta(const void* o, const void* lo, const void
   return 0;
 }
 
-// Gradients of the above: dq [B, Tq, H, D], dk and dv [B, Tk, Hkv, D] contiguous; dq, or dk and dv together, may be null.
+namespace {
+// Parts of a key tile's walk: with fewer key tiles than two blocks an SM, as many as make up two, of two tiles of rows each at least.
+int parts_of(int B, int H, int Hkv, int Tq, int Tk, int D) {
+  const long long BT = D <= 128 ? 64 : 32, units = (Tk + BT - 1) / BT * Hkv * B, blocks = 2ll * kb_sm_count(), walk = (long long)(H / Hkv) * ((Tq + BT - 1) / BT);
+  if (units >= blocks) return 1;
+  const long long want = (blocks + units - 1) / units, most = walk / 2 < 16 ? walk / 2 : 16;
+  return (int)(want < most ? want : most > 1 ? most : 1);
+}
+}  // namespace
+
+// Floats of workspace that kb200_attention_rules_bwd takes for dk and dv at these sizes.
+KB_API long long kb200_attention_rules_bwd_work_plain(int B, int H, int Hkv, int Tq, int Tk, int D) {
+  if (B <= 0 || Hkv <= 0 || H < Hkv || Tq <= 0 || Tk <= 0 || D <= 0) return 0;
+  const int parts = parts_of(B, H, Hkv, Tq, Tk, D);
+  return parts > 1 ? 2ll * parts * B * Tk * Hkv * D : 0;
+}
+
+// Gradients of the above: dq [B, Tq, H, D], dk and dv [B, Tk, Hkv, D] contiguous; dq, or dk and dv together, may be null.  work: `floats` of them, as many as
+// kb200_attention_rules_bwd_work_plain says, or null.
 KB_API int kb200_attention_rules_bwd(const void* q, const void* k, const void* v, const void* grad_out, const long long* strides, const float* lse, const float* delta, int pitch,
-                                     void* dq, void* dk, void* dv, int dtype, int B, int H, int Hkv, int Tq, int Tk, int D, float scale, float cap, const float* slopes, int causal, int window,
+                                     void* dq, void* dk, void* dv, int dtype, int B, int H, int Hkv, int Tq, int Tk, int D, float* work, long long floats, float scale, float cap, const float* slopes, int causal, int window,
                                      const int* prefix, const int* seg_q, const int* seg_k, const void* range_q, const void* range_k, cudaStream_t stream) {
   const Rules r{B, H, Hkv, Tq, Tk, D, scale, cap, slopes, causal, window, prefix, seg_q, seg_k, (const int4*)range_q, (const int4*)range_k};
   if (!check(r, dtype)) return -2;
   const Strides qs{strides[0], strides[1], strides[2]}, ks{strides[3], strides[4], strides[5]}, vs{strides[6], strides[7], strides[8]};
   const Gradients g{grad_out, {strides[9], strides[10], strides[11]}, lse, delta, pitch};
+  Parts parts{parts_of(B, H, Hkv, Tq, Tk, D), work};
+  if (work == nullptr || 2ll * parts.count * B * Tk * Hkv * D > floats) parts.count = 1;
   int rc = 0;
-#define KB_CALL(T, DP, BT) rules_bwd<T, DP, BT>(r, q, qs, k, ks, v, vs, g, dq, dk, dv, stream)
+#define KB_CALL(T, DP, BT) rules_bwd<T, DP, BT>(r, q, qs, k, ks, v, vs, g, dq, dk, dv, parts, stream)
   KB_RULES_DISPATCH(KB_CALL);
 #undef KB_CALL
   if (rc != 0) return rc;
@@ -598,12 +654,12 @@ KB_API int kb200_attention_rules_bwd(const void* q, const void* k, const void* v
 
 // All of a gradient in one call: delta, from o, lo (may be null) and grad_out, then the above.  err is unused.
 KB_API int kb200_attention_rules_grads(const void* q, const void* k, const void* v, const void* o, const void* lo, const void* grad_out, const long long* strides, const float* lse,
-                                       float* delta, int pitch, void* dq, void* dk, void* dv, int dtype, int B, int H, int Hkv, int Tq, int Tk, int D, int* err, float scale, float cap,
+                                       float* delta, int pitch, void* dq, void* dk, void* dv, int dtype, int B, int H, int Hkv, int Tq, int Tk, int D, int* err, float* work, long long floats, float scale, float cap,
                                        const float* slopes, int causal, int window, const int* prefix, const int* seg_q, const int* seg_k, const void* range_q, const void* range_k,
                                        cudaStream_t stream) {
   (void)err;
   const int rc = kb200_attention_rules_delta(o, lo, grad_out, strides + 9, delta, pitch, dtype, B, H, Tq, D, stream);
   return rc != 0 ? rc
-                 : kb200_attention_rules_bwd(q, k, v, grad_out, strides, lse, delta, pitch, dq, dk, dv, dtype, B, H, Hkv, Tq, Tk, D, scale, cap, slopes, causal, window, prefix, seg_q,
+                 : kb200_attention_rules_bwd(q, k, v, grad_out, strides, lse, delta, pitch, dq, dk, dv, dtype, B, H, Hkv, Tq, Tk, D, work, floats, scale, cap, slopes, causal, window, prefix, seg_q,
                                              seg_k, range_q, range_k, stream);
 }

@@ -14,6 +14,8 @@
 // exponential each, about 1000 cycles for two warps a scheduler, twice that with a cap.
 //
 // Every mbarrier wait is bounded; on expiry the kernel writes a code to *err, lets its copies land, frees TMEM and returns.
+#include <algorithm>
+
 #include "attention_rules_sm100.cuh"
 
 namespace {
@@ -61,6 +63,45 @@ __device__ __forceinline__ void probabilities(float (&x)[32], float (&w)[32], co
   }
 }
 
+// A key tile's walk over the query heads of its group and their row tiles, and the part of it that a CTA takes.
+struct Parts {
+  int count;    // parts of a key tile; 1: its gradients are stored as they are
+  float* sums;  // [dk, dv][count][B, Tk, Hkv, D]
+};
+
+// 32 columns of a row in float32, or zeros.
+__device__ __forceinline__ void store_sums(float* to, uint32_t tmem, int col, int D, bool valid, bool zero) {
+  float o[32];
+  if (!zero) {
+    tmem_ld32(tmem, reinterpret_cast<uint32_t*>(o));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  }
+#pragma unroll
+  for (int u = 0; u < 8; ++u)
+    if (valid && col + u * 4 < D)
+      *reinterpret_cast<float4*>(to + col + u * 4) = zero ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[u * 4], o[u * 4 + 1], o[u * 4 + 2], o[u * 4 + 3]);
+}
+
+// dk and dv from the sums of their parts, in order.
+template <typename T>
+__global__ void __launch_bounds__(256) join_parts_kernel(const float4* sums, T* dk, T* dv, int parts, long long n, float scale) {
+  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (at >= 2 * n) return;
+  const bool second = at >= n;
+  const long long e = second ? at - n : at;
+  const float4* from = sums + (second ? (long long)parts * n : 0) + e;
+  float4 x = from[0];
+  for (int i = 1; i < parts; ++i) {
+    const float4 y = from[i * n];
+    x.x += y.x;
+    x.y += y.y;
+    x.z += y.z;
+    x.w += y.w;
+  }
+  const float f = second ? 1.f : scale;
+  reinterpret_cast<uint2*>(second ? dv : dk)[e] = make_uint2(pack_16<T>(x.x * f, x.y * f), pack_16<T>(x.z * f, x.w * f));
+}
+
 // Pulls the tail of a 32-column slice of TMEM into 16-byte stores of one row.
 template <typename T>
 __device__ __forceinline__ void store_row(T* to, uint32_t tmem, int col, int D, float factor, bool valid, bool zero) {
@@ -90,7 +131,7 @@ struct DkvCfg {
 template <typename T, int D>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
 rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                const __grid_constant__ CUtensorMap map_g, const Rules p, const Cap c_, const Sums sums, T* dk, T* dv, int* err) {
+                const __grid_constant__ CUtensorMap map_g, const Rules p, const Cap c_, const Sums sums, T* dk, T* dv, const Parts parts, int* err) {
   using C = DkvCfg<D>;
   constexpr int TILE = C::TILE, ST = C::STAGES;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -108,14 +149,24 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int groups = p.Hkv * p.B, k0 = (int)(blockIdx.x / groups) * BLK;  // a causal mask gives the first keys the most rows
-  const int hkv = (int)(blockIdx.x % groups) % p.Hkv, b = (int)(blockIdx.x % groups) / p.Hkv, group = p.H / p.Hkv;
+  const int unit = (int)(blockIdx.x / parts.count), part = (int)(blockIdx.x % parts.count);
+  const int groups = p.Hkv * p.B, k0 = unit / groups * BLK;  // a causal mask gives the first keys the most rows
+  const int hkv = unit % groups % p.Hkv, b = unit % groups / p.Hkv, group = p.H / p.Hkv;
   const int prefix = p.prefix != nullptr ? p.prefix[b] : 0;
   int first, last;  // tiles of rows
   rows_of_keys(p, k0, min(k0 + BLK, p.Tk) - 1, prefix, first, last);
   first /= BLK;
   last = last < 0 ? -1 : last / BLK;
-  for (int n = threadIdx.x; first + n <= last; n += BWD_THREADS) flags[n] = (uint8_t)tile_flags(p, b, (first + n) * BLK, k0, prefix);
+  int* n_needed = reinterpret_cast<int*>(smem_raw + C::BARS + 64 + 16 * ST);
+  if (threadIdx.x == 0) *n_needed = 0;
+  __syncthreads();
+  int needed = 0;
+  for (int n = threadIdx.x; first + n <= last; n += BWD_THREADS) {
+    const int f = tile_flags(p, b, (first + n) * BLK, k0, prefix);
+    flags[n] = (uint8_t)f;
+    needed += f & NEEDED;
+  }
+  if (needed > 0) atomicAdd(n_needed, needed);
   const int end = last - first + 1;
   auto next = [&](int n) {
     do ++n;
@@ -145,30 +196,37 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
   const uint32_t tS = tmem, tP = tmem + 128, tV = tmem + 256, tK = tmem + 256 + D;
-  const int start = next(-1);
+  // this part's share of the walk: `mine` tiles from head `g0` and row tile `n0` on
+  const int per_head = *n_needed, total = per_head * group, per = (total + parts.count - 1) / parts.count;
+  const int mine = max(0, min(total - part * per, per)), start = next(-1);
+  int g0 = 0, n0 = start;
+  if (mine > 0) {
+    g0 = part * per / per_head;
+    for (int skip = part * per % per_head; skip > 0; --skip) n0 = next(n0);
+  }
 
   if (warp < 16) {
     // ------------------------------------------------------------------ scores: a lane a key, 32 of its rows
-    const int part = warp >> 2, key = k0 + (warp & 3) * 32 + lane;
-    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, at = lane_base + (uint32_t)(part * 32);
+    const int quarter = warp >> 2, key = k0 + (warp & 3) * 32 + lane;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, at = lane_base + (uint32_t)(quarter * 32);
     const bool cap = p.cap > 0.f;
     int lo, hi, own = 0;
     rows_of_keys(p, key, key, prefix, lo, hi);
     if (key >= p.Tk) hi = -1;
     if (p.seg_k != nullptr) own = key < p.Tk ? p.seg_k[(long long)b * p.Tk + key] : -1;
     bool ok = true;
-    int it = 0;
-    for (int g = 0; g < group && ok; ++g) {
-      const Score f = score_of(p, hkv * group + g);
-      for (int n = start; n < end; n = next(n), ++it) {
-        const int q0 = (first + n) * BLK + part * 32, stage = it % ST;
+    int it = 0, g = g0, n = n0;
+    Score f = score_of(p, hkv * group + g);
+    {
+      for (; it < mine && ok; ++it) {
+        const int q0 = (first + n) * BLK + quarter * 32, stage = it % ST;
         const bool whole = flags[n] & WHOLE;
         uint32_t keep = ~0u;
         if (!whole) {
           keep = span_bits(lo, hi, q0);
           if (p.seg_q != nullptr) keep &= segment_bits(q0 + lane < p.Tq ? p.seg_q[(long long)b * p.Tq + q0 + lane] : -1, own);
         }
-        const float* lse = reinterpret_cast<const float*>(smem_raw + C::SUMS + stage * 1024) + part * 32;
+        const float* lse = reinterpret_cast<const float*>(smem_raw + C::SUMS + stage * 1024) + quarter * 32;
         ok = mbar_wait(full(stage), (it / ST) & 1, abort_flag) && mbar_wait(s_full, it & 1, abort_flag);
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -201,24 +259,34 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(ds_ready);
+        if ((n = next(n)) >= end && it + 1 < mine) {
+          n = start;
+          f = score_of(p, hkv * group + ++g);
+        }
       }
     }
     if (ok && it > 0) {
       ok = __all_sync(0xffffffffu, mbar_wait(all_done, 0, abort_flag));
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     }
-    if (ok) {  // half of the warps store dV, the others dK, each half of the columns
-      T* to = (part < 2 ? dv : dk) + (((long long)b * p.Tk + min(key, p.Tk - 1)) * p.Hkv + hkv) * p.D;
+    if (ok && parts.count > 1) {
+      const long long row = (((long long)b * p.Tk + min(key, p.Tk - 1)) * p.Hkv + hkv) * p.D, size = (long long)p.B * p.Tk * p.Hkv * p.D;
+      float* to = parts.sums + (quarter < 2 ? (long long)parts.count * size : 0) + part * size + row;
 #pragma unroll 1
-      for (int c = (part & 1) * (D / 2); c < ((part & 1) + 1) * (D / 2); c += 32)
-        store_row(to, (part < 2 ? tV : tK) + lane_base + (uint32_t)c, c, p.D, part < 2 ? 1.f : p.scale, key < p.Tk, it == 0);
+      for (int c = (quarter & 1) * (D / 2); c < ((quarter & 1) + 1) * (D / 2); c += 32)
+        store_sums(to, (quarter < 2 ? tV : tK) + lane_base + (uint32_t)c, c, p.D, key < p.Tk, mine == 0);
+    } else if (ok) {  // half of the warps store dV, the others dK, each half of the columns
+      T* to = (quarter < 2 ? dv : dk) + (((long long)b * p.Tk + min(key, p.Tk - 1)) * p.Hkv + hkv) * p.D;
+#pragma unroll 1
+      for (int c = (quarter & 1) * (D / 2); c < ((quarter & 1) + 1) * (D / 2); c += 32)
+        store_row(to, (quarter < 2 ? tV : tK) + lane_base + (uint32_t)c, c, p.D, quarter < 2 ? 1.f : p.scale, key < p.Tk, it == 0);
     } else {
       if (lane == 0 && err) atomicExch(err, 53);
       *abort_flag = 1;
     }
   } else if (warp == 16) {
     // ------------------------------------------------------------------ TMA producer
-    if (elect_one() && start < end) {
+    if (elect_one() && mine > 0) {
       mbar_expect_tx(kv_bar, 2 * TILE);
 #pragma unroll
       for (int c = 0; c < C::CH; ++c) {
@@ -226,10 +294,14 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         tma_load_4d(sV + c * 16384, &map_v, kv_bar, c * 64, k0, hkv, b);
       }
       bool ok = true;
-      int it = 0;
-      for (int g = 0; g < group && ok; ++g) {
-        const int h = hkv * group + g;
-        for (int n = start; n < end; n = next(n), ++it) {
+      int it = 0, g = g0, n = n0;
+      {
+        for (; it < mine; ++it, n = next(n)) {
+          if (n >= end) {
+            n = start;
+            ++g;
+          }
+          const int h = hkv * group + g;
           const int stage = it % ST, q0 = (first + n) * BLK;
           ok = mbar_wait(empty(stage), ((it / ST) & 1) ^ 1, abort_flag);
           if (!ok) break;
@@ -257,7 +329,7 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     }
   } else {
     // ------------------------------------------------------------------ MMA issuer
-    if (elect_one() && start < end) {
+    if (elect_one() && mine > 0) {
       constexpr uint32_t idesc_s = product_desc<T>(128, 128, false), idesc_o = product_desc<T>(128, D, true);
       auto rows = [&](uint32_t to, uint32_t a, uint32_t bb) {  // 128 x 128 over the head dimension
 #pragma unroll
@@ -273,9 +345,6 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         for (int k = 0; k < 8; ++k)
           umma_bf16_ts(to, a + (uint32_t)((k >> 1) * 32 + (k & 1) * 8), bdesc + (uint64_t)((2048u >> 4) * k), idesc_o, (add || k > 0) ? 1u : 0u);
       };
-      int total = 0;
-      for (int n = start; n < end; n = next(n)) ++total;
-      total *= group;
       auto q_of = [&](int it) { return sQG + (uint32_t)((it % ST) * C::STAGE); };
       bool ok = mbar_wait(kv_bar, 0, abort_flag) && mbar_wait(full(0), 0, abort_flag);
       if (ok) {
@@ -285,12 +354,12 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         rows(tP, sV, q_of(0) + TILE);
         umma_commit(dp_full);
       }
-      for (int it = 0; it < total && ok; ++it) {
+      for (int it = 0; it < mine && ok; ++it) {
         ok = mbar_wait(p_ready, it & 1, abort_flag);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         cols(tV, tS, q_of(it) + TILE, it > 0);
-        if (it + 1 < total) {
+        if (it + 1 < mine) {
           ok = mbar_wait(full((it + 1) % ST), ((it + 1) / ST) & 1, abort_flag);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -302,7 +371,7 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         cols(tK, tP, q_of(it), it > 0);
         umma_commit(empty(it % ST));
-        if (it + 1 < total) {
+        if (it + 1 < mine) {
           rows(tP, sV, q_of(it + 1) + TILE);
           umma_commit(dp_full);
         }
@@ -559,10 +628,20 @@ rules_dq_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   if (warp == 17) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
+// Parts that a key tile's walk is split into: with fewer key tiles than SMs (few key heads, whose query heads are all walked over one after the other),
+// as many as fill the chip, of four tiles each at least.  A part of its own costs its start, about three tiles, and its sums in memory.
+int parts_of(int B, int H, int Hkv, int Tq, int Tk) {
+  const long long units = (long long)((Tk + BLK - 1) / BLK) * Hkv * B, sms = kb_sm_count();
+  const long long walk = (long long)(H / Hkv) * ((Tq + BLK - 1) / BLK);
+  if (units >= sms) return 1;
+  const long long want = (sms + units - 1) / units, most = walk / 4;
+  return (int)std::max(1ll, std::min(std::min(want, most), 16ll));
+}
+
 int flag_bytes(int T) { return ((T + BLK - 1) / BLK + 15) / 16 * 16; }
 
 template <typename T, int D>
-int launch_bwd(const CUtensorMap* m, const Rules& p, const Sums& sums, void* dq, void* dk, void* dv, int* err, cudaStream_t stream) {
+int launch_bwd(const CUtensorMap* m, const Rules& p, const Sums& sums, void* dq, void* dk, void* dv, const Parts& parts, int* err, cudaStream_t stream) {
   static bool attr[2][KB_MAX_DEVICES] = {{false}};
   if (!kb_allow_smem(rules_dkv_sm100<T, D>, DkvCfg<D>::FLAGS + MAX_BLOCKS, attr[0]) || !kb_allow_smem(rules_dq_sm100<T, D>, DqCfg<D>::FLAGS + MAX_BLOCKS, attr[1])) {
     kb200_set_error("attention_rules: shared-memory limit");
@@ -570,8 +649,12 @@ int launch_bwd(const CUtensorMap* m, const Rules& p, const Sums& sums, void* dq,
   }
   const Cap cap = make_cap(p.scale, p.cap);
   if (dk != nullptr)
-    rules_dkv_sm100<T, D><<<(unsigned)((long long)((p.Tk + BLK - 1) / BLK) * p.Hkv * p.B), BWD_THREADS, DkvCfg<D>::FLAGS + flag_bytes(p.Tq), stream>>>(m[0], m[1], m[2], m[3], p, cap,
-                                                                                                                                               sums, (T*)dk, (T*)dv, err);
+    rules_dkv_sm100<T, D><<<(unsigned)((long long)((p.Tk + BLK - 1) / BLK) * p.Hkv * p.B * parts.count), BWD_THREADS, DkvCfg<D>::FLAGS + flag_bytes(p.Tq), stream>>>(m[0], m[1], m[2], m[3], p, cap,
+                                                                                                                                               sums, (T*)dk, (T*)dv, parts, err);
+  if (dk != nullptr && parts.count > 1) {
+    const long long n = (long long)p.B * p.Tk * p.Hkv * p.D / 4;
+    join_parts_kernel<T><<<(unsigned)((2 * n + 255) / 256), 256, 0, stream>>>((const float4*)parts.sums, (T*)dk, (T*)dv, parts.count, n, p.scale);
+  }
   if (dq != nullptr)
     rules_dq_sm100<T, D><<<(unsigned)((long long)((p.Tq + BLK - 1) / BLK) * p.H * p.B), BWD_THREADS, DqCfg<D>::FLAGS + flag_bytes(p.Tk), stream>>>(m[0], m[1], m[2], m[3], p, cap, sums,
                                                                                                                                            (T*)dq, err);
@@ -580,10 +663,17 @@ int launch_bwd(const CUtensorMap* m, const Rules& p, const Sums& sums, void* dq,
 
 }  // namespace
 
+// Floats of workspace that kb200_attention_rules_bwd_sm100 takes for dk and dv at these sizes.
+KB_API long long kb200_attention_rules_bwd_work(int B, int H, int Hkv, int Tq, int Tk, int D) {
+  if (B <= 0 || Hkv <= 0 || H < Hkv || Tq <= 0 || Tk <= 0 || D <= 0) return 0;
+  const int parts = parts_of(B, H, Hkv, Tq, Tk);
+  return parts > 1 ? 2ll * parts * B * Tk * Hkv * D : 0;
+}
+
 // As kb200_attention_rules_bwd for what kb200_attention_rules_fwd_sm100 takes, at most 1048576 rows and keys; lse and delta with rows `pitch` apart, a
-// multiple of 128.
+// multiple of 128.  work: `floats` of them, 16-byte aligned, as many as kb200_attention_rules_bwd_work says, or null.
 KB_API int kb200_attention_rules_bwd_sm100(const void* q, const void* k, const void* v, const void* grad_out, const long long* strides, const float* lse, const float* delta,
-                                           int pitch, void* dq, void* dk, void* dv, int dtype, int B, int H, int Hkv, int Tq, int Tk, int D, int* err, float scale, float cap,
+                                           int pitch, void* dq, void* dk, void* dv, int dtype, int B, int H, int Hkv, int Tq, int Tk, int D, int* err, float* work, long long floats, float scale, float cap,
                                            const float* slopes, int causal, int window, const int* prefix, const int* seg_q, const int* seg_k, const void* range_q,
                                            const void* range_k, cudaStream_t stream) {
   const Rules p{B, H, Hkv, Tq, Tk, D, scale, cap, slopes, causal, window, prefix, seg_q, seg_k, (const int4*)range_q, (const int4*)range_k};
@@ -606,9 +696,11 @@ KB_API int kb200_attention_rules_bwd_sm100(const void* q, const void* k, const v
     return -3;
   }
   const Sums sums{lse, delta, pitch};
+  Parts parts{parts_of(B, H, Hkv, Tq, Tk), work};
+  if (work == nullptr || 2ll * parts.count * B * Tk * Hkv * D > floats) parts.count = 1;
   int rc;
-  if (D <= 64) rc = half ? launch_bwd<__half, 64>(m, p, sums, dq, dk, dv, err, stream) : launch_bwd<__nv_bfloat16, 64>(m, p, sums, dq, dk, dv, err, stream);
-  else rc = half ? launch_bwd<__half, 128>(m, p, sums, dq, dk, dv, err, stream) : launch_bwd<__nv_bfloat16, 128>(m, p, sums, dq, dk, dv, err, stream);
+  if (D <= 64) rc = half ? launch_bwd<__half, 64>(m, p, sums, dq, dk, dv, parts, err, stream) : launch_bwd<__nv_bfloat16, 64>(m, p, sums, dq, dk, dv, parts, err, stream);
+  else rc = half ? launch_bwd<__half, 128>(m, p, sums, dq, dk, dv, parts, err, stream) : launch_bwd<__nv_bfloat16, 128>(m, p, sums, dq, dk, dv, parts, err, stream);
   if (rc != 0) return rc;
   KB_CHECK_LAUNCH("attention_rules_bwd_sm100");
   return 0;
@@ -620,10 +712,10 @@ KB_API int kb200_attention_rules_delta(const void* o, const void* lo, const void
 // All of a gradient in one call: delta, from o, lo (may be null) and grad_out, then the above.
 KB_API int kb200_attention_rules_grads_sm100(const void* q, const void* k, const void* v, const void* o, const void* lo, const void* grad_out, const long long* strides,
                                              const float* lse, float* delta, int pitch, void* dq, void* dk, void* dv, int dtype, int B, int H, int Hkv, int Tq, int Tk, int D, int* err,
-                                             float scale, float cap, const float* slopes, int causal, int window, const int* prefix, const int* seg_q, const int* seg_k,
+                                             float* work, long long floats, float scale, float cap, const float* slopes, int causal, int window, const int* prefix, const int* seg_q, const int* seg_k,
                                              const void* range_q, const void* range_k, cudaStream_t stream) {
   const int rc = kb200_attention_rules_delta(o, lo, grad_out, strides + 9, delta, pitch, dtype, B, H, Tq, D, stream);
   return rc != 0 ? rc
-                 : kb200_attention_rules_bwd_sm100(q, k, v, grad_out, strides, lse, delta, pitch, dq, dk, dv, dtype, B, H, Hkv, Tq, Tk, D, err, scale, cap, slopes, causal, window, prefix,
+                 : kb200_attention_rules_bwd_sm100(q, k, v, grad_out, strides, lse, delta, pitch, dq, dk, dv, dtype, B, H, Hkv, Tq, Tk, D, err, work, floats, scale, cap, slopes, causal, window, prefix,
                                                    seg_q, seg_k, range_q, range_k, stream);
 }
