@@ -639,10 +639,14 @@ struct Split {
 Split split_of(const Cache& c, bool tensor) {
   const long long rows = (long long)c.T * (c.H / c.Hkv), pairs = (long long)c.B * c.Hkv;
   Split s{pairs * (tensor && rows <= 8 ? 1 : (rows + 15) / 16), 1, 0};
-  const long long most = ((long long)c.wide * c.page + 127) / 128;  // at least 128 positions a part where the table is full
+  // positions that a row may see, where the table is full
+  const long long full = (long long)c.wide * c.page, seen = c.window > 0 && c.window + (long long)c.T < full ? c.window + (long long)c.T : full;
+  const long long most = (seen + 127) / 128;  // at least 128 positions a part
   const int sms = kb_sm_count();
-  // clusters: as many parts as give every SM about four blocks, which evens out sequences of different lengths
-  while (s.cluster < 8 && s.cluster * 2 <= most && s.units * s.cluster < 4ll * sms) s.cluster *= 2;
+  // clusters: as many parts as give every SM about four blocks, which evens out sequences of different lengths (64 sequences of 200 to 4000: 122 us,
+  // whole 135 us).  Once there is a block for every SM a further part has to be worth its start: 1024 positions (16 sequences within a window of 1024: 40 us
+  // in one part, 49 us in two).
+  while (s.cluster < 8 && s.cluster * 2 <= most && s.units * s.cluster < 4ll * sms && (s.units * s.cluster < sms || s.cluster * 2048ll <= seen)) s.cluster *= 2;
   if (tensor && s.cluster == 8 && s.units * 8 < 3ll * sms && most > 8) {
     // Few long sequences: one wave of three blocks an SM.  (Clusters of eight large blocks, of which the chip holds no more than about half as
     // many as its SMs would allow, took twice the time.)
@@ -712,7 +716,7 @@ bool tensor_cores(const Cache& c, int dtype, const void* k, const void* v, const
 }  // namespace
 
 // Floats of workspace that kb200_attention_cache may use at these sizes.
-KB_API long long kb200_attention_cache_work(int B, int H, int Hkv, int T, int D, int page, int wide) {
+KB_API long long kb200_attention_cache_work(int B, int H, int Hkv, int T, int D, int page, int wide, int window) {
   Cache c{};
   c.B = B;
   c.H = H;
@@ -721,6 +725,7 @@ KB_API long long kb200_attention_cache_work(int B, int H, int Hkv, int T, int D,
   c.D = D;
   c.page = page;
   c.wide = wide;
+  c.window = window;
   if (B <= 0 || T <= 0 || Hkv <= 0 || H < Hkv || D <= 0 || D > 128) return 0;
   return work_of(c, split_of(c, true));
 }
