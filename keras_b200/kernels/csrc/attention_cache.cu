@@ -39,14 +39,22 @@ struct CacheTile {
   static constexpr int FLOATS = ROWS * PITCH + KEYS * PITCH * 2 + ROWS * (KEYS + 1) + 3 * ROWS;
 };
 
+// Parts that do not join within a cluster leave their rows, maxima and sums here; join_kernel adds them up.
+struct Parts {
+  float* rows;  // [units][parts][rows of a unit][D], null: join in the cluster
+  float2* sums; // [units][parts][rows of a unit]: maximum, sum
+  int count;
+};
+
 template <typename T, int DP>
-__global__ void __launch_bounds__(THREADS) cache_kernel(const Cache c, const T* q, const T* new_k, const T* new_v, T* pool_k, T* pool_v, T* out, int vec) {
+__global__ void __launch_bounds__(THREADS) cache_kernel(const Cache c, const T* q, const T* new_k, const T* new_v, T* pool_k, T* pool_v, T* out, const Parts ws, int vec) {
   constexpr int PITCH = CacheTile<DP>::PITCH, COLS = DP / THREADS > 0 ? DP / THREADS : 1;
   extern __shared__ __align__(16) float sm[];
   float *sQ = sm, *sK = sQ + ROWS * PITCH, *sV = sK + KEYS * PITCH, *sP = sV + KEYS * PITCH, *sM = sP + ROWS * (KEYS + 1), *sL = sM + ROWS, *sA = sL + ROWS;
   __shared__ int s_bad[KEYS];
   cg::cluster_group cluster = cg::this_cluster();
-  const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
+  const bool joined = ws.rows == nullptr;
+  const int parts = joined ? (int)cluster.num_blocks() : ws.count, part = (int)(blockIdx.x % parts);
   const int G = c.H / c.Hkv, rows = c.T * G, row_tiles = (rows + ROWS - 1) / ROWS;
   const int unit = (int)(blockIdx.x / parts), rt = unit % row_tiles, hkv = unit / row_tiles % c.Hkv, b = unit / row_tiles / c.Hkv;
   const int r0 = rt * ROWS, nr = min(ROWS, rows - r0);  // row r: token r / G, query head hkv * G + r % G
@@ -171,6 +179,19 @@ __global__ void __launch_bounds__(THREADS) cache_kernel(const Cache c, const T* 
     }
   }
   __syncthreads();
+  if (!joined) {
+    const long long at = ((long long)unit * parts + part) * ROWS;
+#pragma unroll
+    for (int e = 0; e < COLS; ++e) {
+      const int d = tid + e * THREADS;
+      if (d < DP)
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+          if (r < nr) ws.rows[(at + r) * DP + d] = acc[r][e];
+    }
+    if (tid < ROWS) ws.sums[at + tid] = make_float2(sM[tid], sL[tid]);
+    return;
+  }
   // this CTA's part over its query tile: [row][column]
 #pragma unroll
   for (int e = 0; e < COLS; ++e) {
@@ -241,13 +262,6 @@ __device__ __forceinline__ uint4 load_once(const void* p) {
 // What a position that is not there, and a column beyond the head's size, reads: an address is chosen, never a value after its load, or the load
 // would be waited for on the spot.
 __device__ uint4 zero_row[16];  // as long as the widest head
-
-// Parts that do not join within a cluster leave their rows, maxima and sums here; join_kernel adds them up.
-struct Parts {
-  float* rows;  // [units][parts][ROWS][D], null: join in the cluster
-  float2* sums; // [units][parts][ROWS]: maximum, sum
-  int count;
-};
 
 // tanh(x * pre) * post of a lane's four scores, for a warp: the polynomial of tanh_small2's kind where no lane has a value beyond 1/2
 __device__ __forceinline__ void capped4(float (&x)[4], float pre, float post) {
@@ -647,10 +661,11 @@ Split split_of(const Cache& c, bool tensor) {
   // whole 135 us).  Once there is a block for every SM a further part has to be worth its start: 1024 positions (16 sequences within a window of 1024: 40 us
   // in one part, 49 us in two).
   while (s.cluster < 8 && s.cluster * 2 <= most && s.units * s.cluster < 4ll * sms && (s.units * s.cluster < sms || s.cluster * 2048ll <= seen)) s.cluster *= 2;
-  if (tensor && s.cluster == 8 && s.units * 8 < 3ll * sms && most > 8) {
-    // Few long sequences: one wave of three blocks an SM.  (Clusters of eight large blocks, of which the chip holds no more than about half as
+  const int fit = tensor ? 3 : 2;  // blocks an SM
+  if (s.cluster == 8 && s.units * 8 < (long long)fit * sms && most > 8) {
+    // Few long sequences: one wave of three blocks an SM (two of the plain kernel's).  (Clusters of eight large blocks, of which the chip holds no more than about half as
     // many as its SMs would allow, took twice the time.)
-    const long long want = 3ll * sms / s.units;
+    const long long want = (long long)fit * sms / s.units;
     s.spread = (int)(want < most ? want : most);
     if (s.spread > 8) s.cluster = 1;
     else s.spread = 0;
@@ -658,25 +673,25 @@ Split split_of(const Cache& c, bool tensor) {
   return s;
 }
 
-// Floats of the workspace of parts that join through memory.
-long long work_of(const Cache& c, const Split& s) { return s.units * s.spread * ((long long)c.T * (c.H / c.Hkv) <= 8 ? 8 : 16) * ((c.D <= 64 ? 64 : 128) + 2); }
+// Rows that a unit's parts leave, and floats of the workspace of parts that join through memory.
+int rows_of(const Cache& c, bool tensor) { return tensor && (long long)c.T * (c.H / c.Hkv) <= 8 ? 8 : 16; }
+long long work_of(const Cache& c, const Split& s, bool tensor) { return s.units * s.spread * rows_of(c, tensor) * ((c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256) + 2); }
 
 template <typename T, int DP>
 int launch_cache(const Cache& c, const void* q, const void* k, const void* v, void* pk, void* pv, void* out, float* work, long long floats, bool tensor, cudaStream_t stream) {
   Split s = split_of(c, tensor);
+  if (s.spread > 0 && work_of(c, s, tensor) > floats) {  // asked for on another kind of device
+    s.spread = 0;
+    s.cluster = 8;
+  }
+  Parts ws{nullptr, nullptr, s.spread};
+  if (s.spread > 0) {
+    ws.sums = reinterpret_cast<float2*>(work);
+    ws.rows = work + 2 * s.units * s.spread * rows_of(c, tensor);
+  }
   if constexpr (sizeof(T) == 2 && DP <= 128) {
     if (tensor) {
       const bool one = (long long)c.T * (c.H / c.Hkv) <= 8;
-      if (s.spread > 0 && work_of(c, s) > floats) {  // asked for on another kind of device
-        s.spread = 0;
-        s.cluster = 8;
-      }
-      Parts ws{nullptr, nullptr, s.spread};
-      if (s.spread > 0) {
-        const long long rows = s.units * s.spread * (one ? 8 : 16);
-        ws.sums = reinterpret_cast<float2*>(work);
-        ws.rows = work + 2 * rows;
-      }
       const long long blocks = s.units * (s.spread > 0 ? s.spread : s.cluster);
 #define KB_LAUNCH(NT, FULL) \
   launch_parts(cache_kernel_16<T, DP, NT, FULL>, blocks, s.cluster, 128, 0, stream, c, (const T*)q, (const T*)k, (const T*)v, (T*)pk, (T*)pv, (T*)out, (const Parts)ws)
@@ -703,7 +718,9 @@ int launch_cache(const Cache& c, const void* q, const void* k, const void* v, vo
   }
   const int vec = vectors<T>(k, c.k.t, c.k.h, c.k.b, c.D) && vectors<T>(v, c.v.t, c.v.h, c.v.b, c.D) && vectors<T>(pk, c.pool_p, c.pool_t, c.pool_h, c.D) &&
                   vectors<T>(pv, c.pool_p, c.pool_t, c.pool_h, c.D);
-  launch_parts(cache_kernel<T, DP>, s.units * s.cluster, s.cluster, THREADS, SMEM, stream, c, (const T*)q, (const T*)k, (const T*)v, (T*)pk, (T*)pv, (T*)out, vec);
+  launch_parts(cache_kernel<T, DP>, s.units * (s.spread > 0 ? s.spread : s.cluster), s.cluster, THREADS, SMEM, stream, c, (const T*)q, (const T*)k, (const T*)v, (T*)pk, (T*)pv, (T*)out,
+               (const Parts)ws, vec);
+  if (s.spread > 0) join_kernel<T, DP, 2><<<(unsigned)(s.units * 16), DP, 0, stream>>>(c, ws, (T*)out);
   return 0;
 }
 
@@ -726,8 +743,9 @@ KB_API long long kb200_attention_cache_work(int B, int H, int Hkv, int T, int D,
   c.page = page;
   c.wide = wide;
   c.window = window;
-  if (B <= 0 || T <= 0 || Hkv <= 0 || H < Hkv || D <= 0 || D > 128) return 0;
-  return work_of(c, split_of(c, true));
+  if (B <= 0 || T <= 0 || Hkv <= 0 || H < Hkv || D <= 0 || D > 256) return 0;
+  const long long plain = work_of(c, split_of(c, false), false), tensor = D <= 128 ? work_of(c, split_of(c, true), true) : 0;
+  return plain > tensor ? plain : tensor;
 }
 
 // q [B, T, H, D], new_k and new_v [B, T, Hkv, D], pools [n_pages, page, Hkv, D] of common strides, unit stride on D; out [B, T, H, D] contiguous;

@@ -9,7 +9,7 @@
 // What the rules add:
 //   tiles       the flags of every tile of 128 keys (left out / looked at / whole) are worked out once, before the roles part; all of
 //               them walk over the same list.  Documents, windows and prefixes cost what they leave visible.
-//   cap         tanh as a polynomial on the FMA pipe while no score of the warp is beyond half the cap; where a tile is whole and has no slopes, its last
+//   cap         tanh as a polynomial on the FMA pipe while no score of the warp is beyond three quarters of the cap; where a tile is whole and has no slopes, its last
 //               product and the subtraction of the maximum are one multiply-add
 //   distance    where all keys lie behind the rows, slope * |i - j| is slope * e of the key's place in the tile, from a table, and a number of the row
 //   masks       128 bits a row, in tiles that are not whole; segments by comparing with ids that the warp loads once
@@ -278,7 +278,7 @@ rules_fwd_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         if (c < 3) tmem_ld32(tS + 32u * (c + 1), reinterpret_cast<uint32_t*>(x[c + 1]));
         extremes(x[c], m4, top, plain || poly, poly);
       }
-      if (poly && __any_sync(0xffffffffu, top * fabsf(c_.pre) > 0.5f)) {
+      if (poly && __any_sync(0xffffffffu, top * fabsf(c_.pre) > 0.75f)) {
         poly = false;
         m4[0] = m4[1] = m4[2] = m4[3] = -INFINITY;
       }
@@ -308,13 +308,13 @@ rules_fwd_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         }
       }
       const uint64_t minus2 = both(m == -INFINITY ? 0.f : offset - m), scale2 = both(unit);
-      const uint64_t b0 = both(c_.near_raw[0]), b1 = both(c_.near_raw[1]), b2 = both(c_.near_raw[2]), b3 = both(c_.near_raw[3]);
+      const uint64_t b0 = both(c_.mid_raw[0]), b1 = both(c_.mid_raw[1]), b2 = both(c_.mid_raw[2]), b3 = both(c_.mid_raw[3]), b4 = both(c_.mid_raw[4]);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         if (poly)  // tanh's last product and the subtraction of the maximum are one multiply-add
           exponentials<T, TRAIN>(x[c], tS + (uint32_t)(c * 16), l2, [&](uint64_t v) {
             const uint64_t u = mul_f32x2(v, v);
-            return fma_f32x2(fma_f32x2(fma_f32x2(fma_f32x2(b3, u, b2), u, b1), u, b0), v, minus2);
+            return fma_f32x2(fma_f32x2(fma_f32x2(fma_f32x2(fma_f32x2(b4, u, b3), u, b2), u, b1), u, b0), v, minus2);
           });
         else
           exponentials<T, TRAIN>(x[c], tS + (uint32_t)(c * 16), l2, [&](uint64_t v) { return fma_f32x2(v, scale2, minus2); });

@@ -119,6 +119,22 @@ def test_heads_that_share_keys(H, K, D):
     _check(*_inputs(2, 200, 200, H, K, D, torch.bfloat16), dict(is_causal=True, distance_slopes=_slopes(H)))
 
 
+@pytest.mark.parametrize("B,T,S,H,K", [(1, 700, 700, 8, 1), (1, 900, 900, 7, 7), (1, 50, 1500, 16, 2), (2, 1500, 50, 4, 2), (1, 130, 130, 12, 1)])
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.float16, 128), (torch.float32, 64), (torch.bfloat16, 200)], ids=str)
+def test_gradients_of_few_key_heads_are_shared_out(B, T, S, H, K, dtype, D):
+    """Blocks take parts of a key tile's walk over its query heads, whose sums are joined; some parts are empty, some begin within a head."""
+    _check(*_inputs(B, T, S, H, K, D, dtype), dict(is_causal=True, sliding_window=400))
+
+
+@pytest.mark.parametrize("reach", [0.4, 0.7, 0.9, 1.5])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=_names)
+def test_every_form_of_the_cap(reach, dtype):
+    """Scores up to so much of their cap: each form of its tanh, in whole tiles and in masked ones."""
+    q, k, v, do = _inputs(1, 400, 400, 2, 2, 64, dtype)
+    top = torch.einsum("bthd,bshd->bhts", q.float(), k.float()).abs().max().item() / 8.0
+    _check(q, k, v, do, dict(is_causal=True, attn_logits_soft_cap=top / reach))
+
+
 @pytest.mark.parametrize("layout", ["heads_first", "fused", "offset", "expanded", "sliced_heads", "backwards"])
 @pytest.mark.parametrize("dtype", DTYPES, ids=_names)
 def test_layouts(layout, dtype):
@@ -360,6 +376,16 @@ def test_page_sizes(page):
 def test_short_and_long_caches_split_over_many_blocks(B, K, n, wide):
     lengths = [n - 13 * (b % 3) for b in range(B)]
     _check_cached(*_cached(lengths, 1, 64, 2 * K, K, 64, torch.bfloat16, wide=wide), lengths, 1, 64, {})
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.float32, 64), (torch.float32, 128), (torch.bfloat16, 200), (torch.float16, 33)], ids=str)
+@pytest.mark.parametrize("T", [1, 6])
+def test_long_caches_of_other_types_and_sizes(dtype, D, T):
+    """Few long sequences are shared out over the chip by the kernel of every type; one is idle, one short."""
+    lengths = [6000, -1, 130]
+    whole, new, cache = _cached(lengths, T, 24, 4, 2, D, dtype)
+    out = _check_cached(whole, new, cache, lengths, T, 24, dict(attn_logits_soft_cap=9.0, sliding_window=5500), skip=(1,))
+    assert (out[1] == 0).all()
 
 
 def test_idle_sequences_and_missing_pages():
