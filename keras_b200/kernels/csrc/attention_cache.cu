@@ -6,7 +6,8 @@
 //
 // A decoder's step reads each key and value once and does little else, so the cache's bytes bound it.  One sequence and key head is the
 // work of a thread-block cluster: its CTAs take equal parts of the visible positions, each with a running maximum and sum, and join
-// their parts through distributed shared memory: one launch, no workspace, and the same order of sums every time.  The T * H / Hkv rows
+// their parts through distributed shared memory: one launch, no workspace, and the same order of sums every time.  Few long sequences are split
+// into more parts than a cluster has, one wave over the chip, which leave their sums in a workspace for a second launch.  The T * H / Hkv rows
 // that share a key head share its loads.
 //
 // A negative length marks an idle sequence: nothing is written and its rows are zero.  A position whose page is missing (behind the end of
@@ -226,6 +227,9 @@ __global__ void __launch_bounds__(THREADS) cache_kernel(const Cache c, const T* 
 // So keys and values go from memory to the products without shared memory in between, and while one tile is worked on the loads of the next
 // are on their way: 8 KB a warp, 96 KB an SM.  Where a tile lies in one page its address is the same for the whole warp.  No barrier until
 // the warps, and then the cluster's blocks, join their parts.
+// Measured, of 6542 GB/s: two sequences of 65000 positions, 8 key heads of 128, 91 us (5.85 TB/s); 64 of 200 to 4000 122 us (4.4 TB/s: blocks of unequal
+// length in 2.3 waves); 16 of which a window leaves 1024, 5 tokens each, 40 us (3.3 TB/s: 256 blocks on 148 SMs); one of 900 7.2 us, a chain of waits for
+// memory.  With float32 in shared memory and the FMA pipes these took 3037, 1534, 261 and 12 us.
 constexpr int TILE_16 = 16;
 
 template <typename T>

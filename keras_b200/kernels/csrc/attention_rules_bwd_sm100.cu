@@ -10,8 +10,14 @@
 // a key (dkv) or a row (dq), every operand is a tile as TMA brought it: the same tile is read along its rows for one product and across
 // them for the other.  Products run in issue order: S of the next tile may be queued behind the product that reads P from the same columns,
 // while the threads are still busy with dS.
-// What bounds them: four and three products of 128 x 128 x D a tile (D = 128: 2048 and 1536 cycles) against 64 scores a thread with an
-// exponential each, about 1000 cycles for two warps a scheduler, twice that with a cap.
+// With few key heads a key tile's walk over its query heads is shared out to several CTAs, whose float32 sums a second launch adds up in order
+// (6 x 777, 8 query heads on 2, D = 80: dkv 66 -> 44 us).
+//
+// What bounds them: a tile's chain of product, exponentials, product, gradient, product, of which only the ends overlap with the next tile's: about
+// 2300 cycles at D = 128, 3000 with a cap, against 2048 and 1536 of products and 1024 of exponentials.  Both TMEM and shared memory are full, so that
+// there is no second CTA to fill the gaps.  Measured at 2 x 4096 x 32/8 x 128: dkv 535 us (1030 TFLOP/s), dq 395 us (1040 TFLOP/s), with a cap 602
+// and 466 us; at 8 x 2048 x 16 x 128 with slopes 372 and 275 us; in a window of 1024 at 8192 x 32/8 x 128 396 and 300 us.  An issuer that walks as a whole
+// warp, and distances without their absolute value, made no difference.
 //
 // Every mbarrier wait is bounded; on expiry the kernel writes a code to *err, lets its copies land, frees TMEM and returns.
 #include <algorithm>
