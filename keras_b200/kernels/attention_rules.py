@@ -167,8 +167,9 @@ def forward(q, k, v, rules, ranges, training, plan=None):
     return out, lse, None
 
 
-def backward(q, k, v, out, lo, lse, grad_out, rules, ranges, want_q, want_kv, plan=None):
-    plan = plan or plan_of(q, k, v)
+def backward(q, k, v, out, lo, lse, grad_out, rules, ranges, want_q, want_kv):
+    q, k, v, out = unit(q), unit(k), unit(v), out.contiguous()
+    plan = plan_of(q, k, v)  # of the tensors as they are now: what was saved may have come back in another layout
     tensor = plan.tensor
     a, b, c, d = q.data_ptr(), k.data_ptr(), v.data_ptr(), grad_out.data_ptr()
     layout = plan.grad_strides
@@ -205,7 +206,7 @@ class RuleAttention(torch.autograd.Function):
         out, lse, lo = forward(q, k, v, rules, ranges, True, plan)
         # the rules' tensors are saved too: one that is written to before the backward pass is an error, as for any operand
         ctx.save_for_backward(q, k, v, out, lo, lse, *ranges, slopes, prefix, rows, keys)
-        ctx.rules, ctx.plain, ctx.plan = Rules(rules.scale, rules.cap, None, rules.causal, rules.window, None, None), plain, plan
+        ctx.rules, ctx.plain = Rules(rules.scale, rules.cap, None, rules.causal, rules.window, None, None), plain
         return out
 
     @staticmethod
@@ -219,7 +220,7 @@ class RuleAttention(torch.autograd.Function):
             given = iter(torch.autograd.grad(ctx.plain(q, k, v, rules), wanted, grad_out, create_graph=True))
             grads = [next(given) if n else None for n in need[:3]]
         else:
-            dq, dk, dv = backward(q, k, v, out, lo, lse, grad_out, rules, (range_q, range_k), need[0], need[1] or need[2], ctx.plan)
+            dq, dk, dv = backward(q, k, v, out, lo, lse, grad_out, rules, (range_q, range_k), need[0], need[1] or need[2])
             grads = [dq, dk if need[1] else None, dv if need[2] else None]
         return (*grads, None, None, None, None, None, None, None)
 

@@ -62,7 +62,8 @@ __global__ void __launch_bounds__(THREADS) cache_kernel(const Cache c, const T* 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long n = c.lengths[b];
   const long long last = n < 0 ? -1 : n + (r0 + nr - 1) / G;  // of the positions that any row sees
-  const long long first = n < 0 ? 0 : c.window > 0 ? max(0ll, n + r0 / G - c.window + 1) : 0;
+  // a length behind the table's end: every row sees its own position, which has no page, and is NaN, whatever there is before
+  const long long first = n < 0 ? 0 : n >= (long long)c.wide * c.page ? n + r0 / G : c.window > 0 ? max(0ll, n + r0 / G - c.window + 1) : 0;
   // parts of whole tiles
   const long long tiles = (last - first + KEYS) / KEYS, per = (tiles + parts - 1) / parts;
   const long long from = first + part * per * KEYS, to = min(last, from + per * KEYS - 1);
@@ -306,7 +307,8 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) cache_kernel_16(const Ca
   const uint32_t last = n + (uint32_t)((r0 + nr - 1) / G), low = n + (uint32_t)(r0 / G);  // what the last and the first token see
   const uint32_t window = c.window > 0 ? (uint32_t)c.window : 0xffffffffu;
   // tiles begin at multiples of 16, so that one of a page of a multiple of 16 lies within it
-  const uint32_t first = low >= window ? (low + 1u - window) / TILE_16 * TILE_16 : 0u;
+  // (a length behind the table's end: every row sees its own position, which has no page, and is NaN, whatever there is before)
+  const uint32_t first = (long long)n >= (long long)c.wide * c.page ? low / TILE_16 * TILE_16 : low >= window ? (low + 1u - window) / TILE_16 * TILE_16 : 0u;
   const uint32_t tiles = idle ? 0u : (last - first) / TILE_16 + 1u, per = (tiles + parts - 1) / parts;
   const uint32_t t0 = part * per;
   const int mine = (int)min(tiles > t0 ? tiles - t0 : 0u, per) - warp;  // this warp takes t0 + warp, t0 + warp + W, ..

@@ -248,7 +248,7 @@ rules_fwd_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     if (p.seg_q != nullptr) own = qi < p.Tq ? p.seg_q[(long long)b * p.Tq + qi] : -1;
     float m = -INFINITY;  // maximum that P is relative to, in log2
     uint64_t l2[2] = {0, 0};
-    const bool short_cap = cap && f.slope == 0.f && c_.folds;
+    const bool short_cap = cap && f.slope == 0.f && c_.folds && p.scale > 0.f;
     bool ok = true;
     int count = 0;  // tiles so far
     for (int n = next(-1); n < end; n = next(n)) {

@@ -171,6 +171,29 @@ def test_scores_beyond_the_cap_and_scales_of_any_sign(dtype):
             definition.check(name, got, found)
 
 
+@pytest.mark.parametrize("scale", [-0.2, -0.01, 0.0])
+def test_a_cap_with_scales_of_any_sign(scale):
+    """Whole tiles and masked ones: with a negative scale the largest score is that of the smallest product."""
+    q, k, v, do = _inputs(1, 400, 400, 2, 2, 64, torch.bfloat16, q_scale=6.0)
+    found = _definition(q, k, v, do, dict(attn_logits_soft_cap=30.0, is_causal=True), scale=scale)
+    for name, got in zip(("out", "dq", "dk", "dv", "out"), _run(q, k, v, do, dict(attn_logits_soft_cap=30.0, is_causal=True, scale=scale))):
+        definition.check(name, got, found)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=_names)
+def test_saved_tensors_that_come_back_in_another_layout(dtype):
+    """Hooks may keep what is saved elsewhere and hand it back contiguous: the gradients go by the tensors they get."""
+    q, k, v, do = (t.transpose(1, 2).contiguous().transpose(1, 2) for t in _inputs(2, 150, 150, 4, 2, 64, dtype))
+    rules = dict(is_causal=True, attn_logits_soft_cap=5.0)
+    want = _run(q, k, v, do, rules)[1:4]
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    assert not leaves[0].is_contiguous()
+    with torch.autograd.graph.save_on_cpu():
+        out = keras.ops.dot_product_attention(*leaves, **rules)
+    for a, b in zip(torch.autograd.grad(out, leaves, do), want):
+        assert torch.equal(a, b)
+
+
 @pytest.fixture(autouse=True)
 def _no_wait_ran_out():
     yield
@@ -410,6 +433,19 @@ def test_idle_sequences_and_missing_pages():
     # within a window that does not reach the missing page its sequence is whole again
     out = keras.ops.dot_product_attention(*new, cache=cache, sliding_window=20)
     assert torch.isfinite(out[2]).all() and torch.isnan(out[3]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=_names)
+@pytest.mark.parametrize("n", [64, 1000, 2 ** 31 - 9])
+def test_lengths_behind_the_table(dtype, n):
+    """Nothing is read or written there: the rows are NaN, at once, however long the sequence is said to be; others are as they were."""
+    whole, new, cache = _cached([50, 20], 2, 16, 4, 2, 64, dtype, wide=4)
+    cache["lengths"][0] = n
+    before = {k: cache[k].clone() for k in ("key", "value")}
+    out = keras.ops.dot_product_attention(*new, cache=cache)
+    assert torch.isnan(out[0]).all() and torch.isfinite(out[1]).all()
+    changed = sum(int((cache[k] != before[k]).logical_and(~(cache[k].isnan() & before[k].isnan())).any(dim=(2, 3)).sum()) for k in before)
+    assert changed <= 4  # the second sequence's two tokens
 
 
 def test_a_cache_of_other_strides_and_past_32_bits():
