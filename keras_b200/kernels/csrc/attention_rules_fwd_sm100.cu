@@ -16,7 +16,8 @@
 // A row that sees nothing keeps a maximum of -inf and becomes zero.
 //
 // What bounds it: an exponential a score, 2048 cycles a pair of tiles on the special-function pipe, and products of about 2800 (operands from
-// shared memory).  A share of the exponentials as a polynomial on the FMA pipe made it slower: with two warps a scheduler its longer chains show.
+// shared memory) at the least; no pipe is busy for more than half of the time, and what lasts is a tile's chain of product, scores, exponentials and product, of
+// which the two CTAs overlap a part.  A share of the exponentials as a polynomial on the FMA pipe made it slower: with two warps a scheduler its longer chains show.
 //
 // For training the CTA stores L = max + log2(sum) of each row, and P goes to the product with the values in two parts, itself in 16 bits and
 // what that rounding lost (the columns are free: P takes half of the scores').  O is then exact to float32 but for its own rounding, and what
