@@ -231,6 +231,8 @@ def attend_cached(q, k, v, cache, scale, cap, distance_slopes, sliding_window, k
     if k.shape != v.shape or q.shape[1] != k.shape[1]:
         _refuse("with a cache, query, key and value are those of the same new tokens, and keys and values of one size. "
                 f"Received: query.shape={tuple(q.shape)}, key.shape={tuple(k.shape)}, value.shape={tuple(v.shape)}")
+    if not q.device == k.device == v.device:  # the kernels read all three by their address on the query's device
+        _refuse(f"query, key and value have to be on one device. Received: {q.device}, {k.device} and {v.device}")
     pool_k, pool_v, pages, lengths = _cache_parts(cache, q, k, v)
     rules = Rules(float(scale), None if cap is None else soft_cap(cap), None if distance_slopes is None else slopes(distance_slopes, q.shape[2], q.device), True,
                   None if sliding_window is None else window(sliding_window), None, None)

@@ -210,6 +210,15 @@ def test_refused_together_with_a_cache():
             keras.ops.dot_product_attention(*new, cache=cache, **extra)
 
 
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_refused_devices_with_a_cache(which):
+    """An operand of another device than the rest's: its address means nothing to a kernel."""
+    _, new, cache = _cached([5, 5], 1, 4)
+    new[which] = new[which].to("meta")
+    with pytest.raises(ValueError, match="device"):
+        keras.ops.dot_product_attention(*new, cache=cache)
+
+
 # ------------------------------------------------------------------------------------------------ layers
 def _layer(kind, **more):
     if kind == "mha":

@@ -448,6 +448,19 @@ def test_lengths_behind_the_table(dtype, n):
     assert changed <= 4  # the second sequence's two tokens
 
 
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_operands_of_the_host_are_refused(which):
+    """Before a launch: a kernel would read the host's address."""
+    _, new, cache = _cached([5, 9], 1, 16, 4, 2, 64, torch.bfloat16)
+    before = {n: cache[n].clone() for n in ("key", "value")}
+    new[which] = new[which].cpu()
+    launches = kops.launch_count()
+    with pytest.raises(ValueError, match="device"):
+        keras.ops.dot_product_attention(*new, cache=cache)
+    assert kops.launch_count() == launches
+    assert all(torch.equal(cache[n].nan_to_num(), before[n].nan_to_num()) for n in before)
+
+
 def test_a_cache_of_other_strides_and_past_32_bits():
     """A pool inside of a larger buffer, whose last pages lie past 2^31 elements."""
     lengths = [100]
