@@ -130,7 +130,7 @@ def plain(q, k, v, rules, bias=None, mask=None):
     S, K = k.shape[1], k.shape[2]
     qh, kh, vh = (t.to(wide).transpose(1, 2) for t in (q, k, v))
     if K != H:
-        kh, vh = (t.repeat_interleave(H // K, dim=1) for t in (kh, vh))
+        kh, vh = (t.repeat_interleave(int(H // K), dim=1) for t in (kh, vh))  # a trace's sizes are tensors of the host
     x = torch.matmul(qh, kh.transpose(-1, -2)) * rules.scale
     if rules.cap is not None:
         x = rules.cap * torch.tanh(x / rules.cap)
@@ -216,7 +216,7 @@ def _plain_cached(q, k, v, pool_k, pool_v, pages, lengths, rules):
     taken = torch.where(there, pages, torch.zeros_like(pages)).long()
     ks, vs = (pool[taken].reshape(B, S, K, D) for pool in (pool_k, pool_v))
     used = seen.any(dim=1)[:, :, None, None] & there.repeat_interleave(page, dim=1)[:, :, None, None]
-    ks, vs = (torch.where(used, t, torch.zeros_like(t)).to(wide).transpose(1, 2).repeat_interleave(H // K, dim=1) for t in (ks, vs))
+    ks, vs = (torch.where(used, t, torch.zeros_like(t)).to(wide).transpose(1, 2).repeat_interleave(int(H // K), dim=1) for t in (ks, vs))
     x = torch.matmul(q.to(wide).transpose(1, 2), ks.transpose(-1, -2)) * rules.scale
     if rules.cap is not None:
         x = rules.cap * torch.tanh(x / rules.cap)

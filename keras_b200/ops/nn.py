@@ -753,8 +753,8 @@ def dot_product_attention(query, key, value, bias=None, mask=None, scale=None, i
     qh, kh, vh = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
     if attn_logits_soft_cap is not None:
         if K != N:
-            kh = kh.repeat_interleave(N // K, dim=1)
-            vh = vh.repeat_interleave(N // K, dim=1)
+            kh = kh.repeat_interleave(int(N // K), dim=1)  # a trace's sizes are tensors of the host
+            vh = vh.repeat_interleave(int(N // K), dim=1)
         logits = torch.matmul(qh, kh.transpose(-1, -2)) * scale
         logits = attn_logits_soft_cap * torch.tanh(logits / attn_logits_soft_cap)
         if bias is not None:

@@ -303,6 +303,14 @@ def test_the_cap_alone_on_a_trained_layer():
     assert kops.launch_count() > before and loss == loss
 
 
+@pytest.mark.parametrize("rules", [dict(sliding_window=4), dict(attn_logits_soft_cap=5.0)], ids=["window", "cap"])
+def test_shared_key_heads_under_a_trace(rules):
+    q, k, v, _ = _inputs(2, 9, 9, 4, 2, 8, torch.float32)
+    traced = torch.jit.trace(lambda *t: keras.ops.dot_product_attention(*t, is_causal=True, **rules), (q, k, v), check_trace=False)
+    want = _definition(q, k, v, None, dict(rules, is_causal=True))
+    definition.check("out", traced(q, k, v), want)
+
+
 # ------------------------------------------------------------------------------------------------ the paged cache
 def _cached(lengths, T, page, H, K, D, dtype, seed=0, wide=None):
     B, S = len(lengths), max(max(lengths), 0) + T
