@@ -180,10 +180,15 @@ _tracing_state = torch._C._get_tracing_state
 _exporting = torch.compiler.is_exporting
 
 
+def inside_transform():
+    """Inside a transform of ``torch.func``, ``torch.jit.trace`` or ``torch.export``: a tensor that is made here may belong to it alone."""
+    return _in_function_transform() or _tracing_state() is not None or _exporting()
+
+
 def fused_kernels_enabled():
     """False when ``KERAS_B200_DISABLE_FUSED_KERNELS=1``, and inside the transforms of ``torch.func``, forward-mode derivatives, ``torch.jit.trace`` and
     ``torch.export``, which kernels that work on raw pointers cannot take part in: every op then runs its library path."""
-    if _forward_ad._current_level >= 0 or _in_function_transform() or _tracing_state() is not None or _exporting():
+    if _forward_ad._current_level >= 0 or inside_transform():
         return False
     return os.environ.get("KERAS_B200_DISABLE_FUSED_KERNELS", "0") != "1"
 

@@ -81,14 +81,19 @@ def _rules_config(layer):
 
 
 def _slopes_of(layer, like):
-    """The layer's slopes on the device of a tensor: made once a device, so that a recorded step copies nothing from the host."""
+    """The layer's slopes on the device of a tensor: made once a device, so that a recorded step copies nothing from the host.  One that belongs to
+    the mode it was made in (a trace's, an export's, a function transform's) serves its call and is not kept; none is made in inference mode, so that
+    the gradients of a later call can save it."""
     if layer._distance_slopes is None:
         return None
     if not isinstance(like, torch.Tensor) or like.device.type == "meta":
         return list(layer._distance_slopes)
     on = layer._slopes_on.get(like.device)
     if on is None:
-        on = layer._slopes_on[like.device] = torch.tensor(layer._distance_slopes, dtype=torch.float32, device=like.device)
+        with torch.inference_mode(False):
+            on = torch.tensor(layer._distance_slopes, dtype=torch.float32, device=like.device)
+        if type(on) is torch.Tensor and not config.inside_transform():
+            layer._slopes_on[like.device] = on
     return on
 
 

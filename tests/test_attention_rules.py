@@ -330,3 +330,60 @@ def test_rules_in_a_functional_model_that_trains():
     before = [w.copy() for w in model.get_weights()]
     model.train_on_batch(data, rng.normal(size=(4, 8, 3)).astype("float32"))
     assert all(np.isfinite(w).all() for w in model.get_weights()) and any((a != b).any() for a, b in zip(before, model.get_weights()))
+
+
+def _slopes_model(kind, seed=0):
+    keras.utils.set_random_seed(seed)
+    x = keras.Input((8, 16))
+    layer = _layer(kind, distance_slopes=SLOPES)
+    model = keras.Model(x, keras.layers.Dense(3)(layer(x, x, use_causal_mask=True)))
+    model.compile(optimizer="sgd", loss="mse")
+    return model, layer
+
+
+def _transform(how, model, layer, path):
+    """A first call of the layer in a mode whose tensors do not outlive it."""
+    x = torch.randn(2, 8, 16, generator=torch.Generator().manual_seed(5)).to(model.trainable_variables[0].value.device)
+    if how == "export":
+        model.export(str(path / "m"), format="torch_export", verbose=False)
+    elif how == "func_grad":
+        torch.func.grad(lambda z: layer(z, z, use_causal_mask=True).sum())(x)
+    elif how == "vmap":
+        torch.vmap(lambda z: layer(z[None], z[None], use_causal_mask=True))(x)
+    elif how == "trace":
+        for v in layer.trainable_variables:  # a trace holds weights as constants
+            v._value.requires_grad_(False)
+        torch.jit.trace(lambda z: layer(z, z, use_causal_mask=True), (x,), check_trace=False)
+        for v in layer.trainable_variables:
+            v._value.requires_grad_(True)
+    else:
+        with torch.inference_mode():
+            layer(x, x, use_causal_mask=True)
+
+
+TRANSFORMS = ["export", "func_grad", "vmap", "trace", "inference"]
+
+
+def _trains_after(kind, how, path):
+    rng = np.random.default_rng(0)
+    x, y = rng.normal(size=(4, 8, 16)).astype("float32"), rng.normal(size=(4, 8, 3)).astype("float32")
+    losses, weights, kept = [], [], []
+    for first in (None, how):
+        model, layer = _slopes_model(kind)
+        if first is not None:
+            _transform(first, model, layer, path)
+        losses.append([float(model.train_on_batch(x, y)) for _ in range(3)])
+        weights.append(model.get_weights())
+        kept.append(list(layer._slopes_on.values()))
+        assert type(model(x)) is torch.Tensor and np.isfinite(model.predict(x, verbose=0)).all()
+    assert losses[0][0] > 0 and losses[0] == losses[1]
+    assert all(np.array_equal(a, b) for a, b in zip(*weights))
+    for t in kept[1]:
+        assert type(t) is torch.Tensor and not t.is_inference() and not torch._C._functorch.is_functorch_wrapped_tensor(t)
+
+
+@pytest.mark.parametrize("how", TRANSFORMS)
+@pytest.mark.parametrize("kind", ["mha", "gqa"])
+def test_slopes_of_a_transform_do_not_outlive_it(kind, how, tmp_path):
+    """A layer that is first called under an export, a function transform, a trace or in inference mode trains as one that was not."""
+    _trains_after(kind, how, tmp_path)

@@ -7,7 +7,7 @@ import torch
 import keras_b200 as keras
 from keras_b200.kernels import attention, attention_cache, attention_rules, ops as kops
 from tests import attention_definition as definition
-from tests.test_attention_rules import SLOPES, _Decoder, _generation
+from tests.test_attention_rules import SLOPES, TRANSFORMS, _Decoder, _generation, _trains_after
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
@@ -309,6 +309,26 @@ def test_shared_key_heads_under_a_trace(rules):
     traced = torch.jit.trace(lambda *t: keras.ops.dot_product_attention(*t, is_causal=True, **rules), (q, k, v), check_trace=False)
     want = _definition(q, k, v, None, dict(rules, is_causal=True))
     definition.check("out", traced(q, k, v), want)
+
+
+def _spy(monkeypatch):
+    """How often the kernels' two directions run from here on."""
+    calls = {"forward": 0, "backward": 0}
+    for name in calls:
+        def spied(*a, _name=name, _fn=getattr(attention_rules, name), **k):
+            calls[_name] += 1
+            return _fn(*a, **k)
+        monkeypatch.setattr(attention_rules, name, spied)
+    return calls
+
+
+@pytest.mark.parametrize("how", TRANSFORMS)
+@pytest.mark.parametrize("kind", ["mha", "gqa"])
+def test_slopes_of_a_transform_do_not_outlive_it(kind, how, tmp_path, monkeypatch):
+    """The kernels take the slopes' address and save them for the gradients: those of a trace, a transform or inference mode have none, or refuse."""
+    calls = _spy(monkeypatch)
+    _trains_after(kind, how, tmp_path)
+    assert calls["backward"] >= 2 and calls["forward"] > calls["backward"]
 
 
 # ------------------------------------------------------------------------------------------------ the paged cache
