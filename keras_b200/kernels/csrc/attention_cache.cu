@@ -306,9 +306,11 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) cache_kernel_16(const Ca
   const bool idle = length < 0;
   const uint32_t last = n + (uint32_t)((r0 + nr - 1) / G), low = n + (uint32_t)(r0 / G);  // what the last and the first token see
   const uint32_t window = c.window > 0 ? (uint32_t)c.window : 0xffffffffu;
-  // tiles begin at multiples of 16, so that one of a page of a multiple of 16 lies within it
-  // (a length behind the table's end: every row sees its own position, which has no page, and is NaN, whatever there is before)
-  const uint32_t first = (long long)n >= (long long)c.wide * c.page ? low / TILE_16 * TILE_16 : low >= window ? (low + 1u - window) / TILE_16 * TILE_16 : 0u;
+  // the first position that any row sees (a length behind the table's end: every row sees its own position, which has no page, and is NaN, whatever
+  // there is before)
+  const uint32_t begin = (long long)n >= (long long)c.wide * c.page ? low : low >= window ? low + 1u - window : 0u;
+  // tiles begin at multiples of 16, so that one of a page of a multiple of 16 lies within it; what a tile has before `begin` is not read
+  const uint32_t first = begin / TILE_16 * TILE_16;
   const uint32_t tiles = idle ? 0u : (last - first) / TILE_16 + 1u, per = (tiles + parts - 1) / parts;
   const uint32_t t0 = part * per;
   const int mine = (int)min(tiles > t0 ? tiles - t0 : 0u, per) - warp;  // this warp takes t0 + warp, t0 + warp + W, ..
@@ -325,7 +327,7 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) cache_kernel_16(const Ca
     ahead_off = p - slot * (uint32_t)c.page;
     ahead = p <= last && slot < (uint32_t)c.wide ? pages[slot] : -1;
   };
-  // where the tile is: one base for all of it, or each position's own (held by the lane of that number; 0: none, 1: in the pool, 2: of the call)
+  // where the tile is: one base for all of it, or each position's own (held by the lane of that number; 0: seen by no row, 1: in the pool, 2: of the call)
   bool whole = false;
   long long base = 0, at = 0;
   int kind = 0;
@@ -334,7 +336,7 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) cache_kernel_16(const Ca
     const bool valid = (unsigned)ahead < (unsigned)c.n_pages;
     const uint32_t p = pos + (lane & 15);
     at = valid ? (long long)ahead * c.pool_p + (long long)ahead_off * c.pool_t + hkv * c.pool_h : 0;
-    kind = p > last ? 0 : !valid ? -1 : p >= n ? 2 : 1;
+    kind = p > last || p < begin ? 0 : !valid ? -1 : p >= n ? 2 : 1;
     missing = 0;
     whole = even && __all_sync(0xffffffffu, kind == 1);
     if (whole) {

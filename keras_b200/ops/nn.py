@@ -715,10 +715,10 @@ def dot_product_attention(query, key, value, bias=None, mask=None, scale=None, i
     ``pages``, int32 ``[B, n]``, the pool's page for the positions ``i * positions`` .. of each sequence; and ``lengths``, int32 ``[B]``, the positions that are
     taken already.  Query, key and value are those of ``T`` new tokens a sequence.  Their keys and values are written to the pools, at
     ``lengths`` .. ``lengths + T - 1``, and token t sees the positions up to ``lengths + t``.  The caller advances ``lengths`` once all layers have run.
-    A negative length marks an idle sequence: nothing is written and its rows are zero.  A position without a page (behind the table's
-    end, or a number that is no page) is neither read nor written: its rows are NaN on a GPU, and an error on the CPU.  Positions behind a
-    sequence's end may hold anything.  Two sequences may share pages that neither writes to.  No gradients; ``bias``, ``mask``, ``segment_ids`` and
-    ``prefix_lengths`` are refused.
+    A negative length marks an idle sequence: nothing is written and its rows are zero.  A position without a page (behind the table's end, or a
+    number that is no page) is neither read nor written: its rows are NaN on a GPU, and an error on the CPU.  Positions behind a sequence's end, and
+    those that the window of its first new token leaves behind, may hold anything.  Two sequences may share pages that neither writes to.  No
+    gradients; ``bias``, ``mask``, ``segment_ids`` and ``prefix_lengths`` are refused.
     """
     q, k, v = _t(query), _t(key), _t(value)
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:

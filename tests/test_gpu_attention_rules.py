@@ -423,6 +423,21 @@ def test_page_sizes(page):
     _check_cached(*_cached(lengths, 2, page, 4, 2, 64, torch.bfloat16), lengths, 2, page, {})
 
 
+@pytest.mark.parametrize("page", [3, 7, 16, 24, 64])
+@pytest.mark.parametrize("T,window,D", [(1, 5, 64), (1, 16, 128), (5, 33, 64), (20, 9, 128), (2, 200, 80)])
+@pytest.mark.parametrize("dtype", DTYPES, ids=_names)
+def test_positions_before_a_window_may_hold_anything(page, T, window, D, dtype):
+    """Their pages may belong to another sequence by now, or to nobody."""
+    lengths = [30, 100, 515, 2, 64]
+    whole, new, cache = _cached(lengths, T, page, 8, 2, D, dtype)
+    pages = cache["pages"].cpu()
+    for b, n in enumerate(lengths):
+        for p in range(max(0, n + 1 - window)):
+            for name in ("key", "value"):
+                cache[name][int(pages[b, p // page]), p % page] = float("nan") if p % 2 else float("inf")
+    _check_cached(whole, new, cache, lengths, T, page, dict(sliding_window=window))
+
+
 @pytest.mark.parametrize("B,K,n,wide", [(1, 1, 20000, None), (1, 8, 5000, None), (2, 2, 3000, 4000), (200, 2, 40, None)])
 def test_short_and_long_caches_split_over_many_blocks(B, K, n, wide):
     lengths = [n - 13 * (b % 3) for b in range(B)]
