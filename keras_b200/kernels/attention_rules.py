@@ -167,9 +167,36 @@ def forward(q, k, v, rules, ranges, training, plan=None):
     return out, lse, None
 
 
+def _plain_rows(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _as_saved(t, dtype, device, count):
+    return t is None or (t.dtype is dtype and t.numel() == count and t.get_device() == device)
+
+
+def _came_back(q, k, v, out, lo, lse, grad_out, rules, ranges):
+    """The plan of the saved tensors as they are now, once hooks have had them: their addresses say nothing of types and sizes."""
+    plan, device, d, n = plan_of(q, k, v), q.get_device(), q.dtype, q.numel()
+    ok = plan.fits and k.get_device() == device and v.get_device() == device and _as_saved(out, d, device, n) and _as_saved(lo, d, device, n) and _as_saved(grad_out, d, device, n)
+    if ok:
+        B, H, _, T, S, _ = plan.sizes
+        ok = _as_saved(lse, torch.float32, device, B * H * plan.pitch) and _as_saved(rules.slopes, torch.float32, device, H) and _as_saved(rules.prefix, torch.int32, device, B)
+        if rules.segments is not None:
+            counts = (B * T, B * S, B * ((T + 127) // 128) * 4, B * ((S + 127) // 128) * 4)
+            ok = ok and all(_as_saved(t, torch.int32, device, c) for t, c in zip((*rules.segments, *ranges), counts))
+    if not ok:
+        raise RuntimeError("attention by rules: a tensor that was saved for the gradients came back with another type, size or device")
+    return plan
+
+
 def backward(q, k, v, out, lo, lse, grad_out, rules, ranges, want_q, want_kv):
-    q, k, v, out = unit(q), unit(k), unit(v), out.contiguous()
-    plan = plan_of(q, k, v)  # of the tensors as they are now: what was saved may have come back in another layout
+    # what was saved may have come back in another layout, and the C entries take strides of q, k, v and the gradient alone
+    q, k, v, out, lo, lse = unit(q), unit(k), unit(v), _plain_rows(out), _plain_rows(lo), _plain_rows(lse)
+    plan = _came_back(q, k, v, out, lo, lse, grad_out, rules, ranges)
+    rules = rules._replace(slopes=_plain_rows(rules.slopes), prefix=_plain_rows(rules.prefix))
+    if rules.segments is not None:
+        rules, ranges = rules._replace(segments=tuple(map(_plain_rows, rules.segments))), tuple(map(_plain_rows, ranges))
     tensor = plan.tensor
     a, b, c, d = q.data_ptr(), k.data_ptr(), v.data_ptr(), grad_out.data_ptr()
     layout = plan.grad_strides

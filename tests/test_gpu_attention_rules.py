@@ -194,6 +194,39 @@ def test_saved_tensors_that_come_back_in_another_layout(dtype):
         assert torch.equal(a, b)
 
 
+def _turned(t):
+    """The same values, with the first and the last dimension's places in memory exchanged."""
+    return t.transpose(0, -1).contiguous().transpose(0, -1) if t.ndim > 1 else torch.stack([t, t], 1)[:, 0]
+
+
+@pytest.mark.parametrize("rule", ["cap_causal", "all"])
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.float16, 128), (torch.float32, 64), (torch.bfloat16, 200)], ids=str)
+def test_every_saved_tensor_may_come_back_in_another_layout(rule, dtype, D):
+    q, k, v, do = _inputs(3, 150, 150, 4, 2, D, dtype)
+    rules = _rules(rule, 3, 150, 4)
+    want = _run(q, k, v, do, rules)[1:4]
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, _turned):
+        out = keras.ops.dot_product_attention(*leaves, **rules)
+        got = torch.autograd.grad(out, leaves, do)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("change", [lambda t: t.half() if t.dtype == torch.float32 else t, lambda t: t[:1], lambda t: t.long() if t.dtype == torch.int32 else t, lambda t: t.cpu()],
+                         ids=["type", "shape", "integers", "device"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=_names)
+def test_saved_tensors_that_come_back_as_others_are_an_error(change, dtype):
+    """Before a launch, which would read them as what they were."""
+    q, k, v, do = _inputs(3, 20, 20, 4, 2, 64, dtype)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+        out = keras.ops.dot_product_attention(*leaves, **_rules("all", 3, 20, 4))
+        launches = kops.launch_count()
+        with pytest.raises(RuntimeError, match="came back"):
+            torch.autograd.grad(out, leaves, do)
+    assert kops.launch_count() == launches
+
+
 @pytest.fixture(autouse=True)
 def _no_wait_ran_out():
     yield
