@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(256) rules_fwd_kernel(const Rules r, const T* 
   const T* vb = v + b * vs.b + hkv * vs.h;
   load_tile<T, DP, BT>(sQ, q + b * qs.b + h * qs.h, qs.t, q0, r.Tq, r.D, vec & 1);
   const Score f = score_of(r, h);
-  const int prefix = r.prefix != nullptr ? r.prefix[b] : 0;
+  const int prefix = prefix_of(r, b);
   int lo[M], hi[M], seg[M], first, last;
   float m[M], l[M], acc[M][DP / 16];
   keys_of_rows(r, q0, min(q0 + BT, r.Tq) - 1, prefix, first, last);
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(256) rules_dkv_kernel(const Rules r, const T* 
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   load_tile<T, DP, BT>(sK, k + b * ks.b + hkv * ks.h, ks.t, k0, r.Tk, r.D, vec & 2);
   load_tile<T, DP, BT>(sV, v + b * vs.b + hkv * vs.h, vs.t, k0, r.Tk, r.D, vec & 4);
-  const int prefix = r.prefix != nullptr ? r.prefix[b] : 0;
+  const int prefix = prefix_of(r, b);
   float ak[M][DP / 16], av[M][DP / 16];
   int seg_k[M];
 #pragma unroll
@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(256) rules_dq_kernel(const Rules r, const T* q
   load_tile<T, DP, BT>(sQ, q + b * qs.b + h * qs.h, qs.t, q0, r.Tq, r.D, vec & 1);
   load_tile<T, DP, BT>(sG, (const T*)g.grad_out + b * g.go.b + h * g.go.h, g.go.t, q0, r.Tq, r.D, vec & 8);
   const Score f = score_of(r, h);
-  const int prefix = r.prefix != nullptr ? r.prefix[b] : 0;
+  const int prefix = prefix_of(r, b);
   int lo[M], hi[M], seg[M], first, last;
   float lse[M], delta[M], acc[M][DP / 16], scale[M];
   keys_of_rows(r, q0, min(q0 + BT, r.Tq) - 1, prefix, first, last);

@@ -75,6 +75,9 @@ __device__ __forceinline__ Score score_of(const Rules& r, int h) {
   return s;
 }
 
+// Keys that a causal mask does not hide; less than none is none (the lowest number less one would wrap around).
+__device__ __forceinline__ int prefix_of(const Rules& r, int b) { return r.prefix != nullptr ? max(r.prefix[b], 0) : 0; }
+
 __device__ __forceinline__ void row_span(const Rules& r, int i, int prefix, int& lo, int& hi) {
   lo = 0;
   hi = r.Tk - 1;

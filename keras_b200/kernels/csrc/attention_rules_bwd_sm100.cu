@@ -158,7 +158,7 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const int unit = (int)(blockIdx.x / parts.count), part = (int)(blockIdx.x % parts.count);
   const int groups = p.Hkv * p.B, k0 = unit / groups * BLK;  // a causal mask gives the first keys the most rows
   const int hkv = unit % groups % p.Hkv, b = unit % groups / p.Hkv, group = p.H / p.Hkv;
-  const int prefix = p.prefix != nullptr ? p.prefix[b] : 0;
+  const int prefix = prefix_of(p, b);
   int first, last;  // tiles of rows
   rows_of_keys(p, k0, min(k0 + BLK, p.Tk) - 1, prefix, first, last);
   first /= BLK;
@@ -431,7 +431,7 @@ rules_dq_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int groups = p.H * p.B, n_q = (p.Tq + BLK - 1) / BLK, q0 = (n_q - 1 - (int)(blockIdx.x / groups)) * BLK;
   const int h = (int)(blockIdx.x % groups) % p.H, b = (int)(blockIdx.x % groups) / p.H, hkv = h / (p.H / p.Hkv);
-  const int prefix = p.prefix != nullptr ? p.prefix[b] : 0;
+  const int prefix = prefix_of(p, b);
   int first, last;  // tiles of keys
   keys_of_rows(p, q0, min(q0 + BLK, p.Tq) - 1, prefix, first, last);
   first /= BLK;

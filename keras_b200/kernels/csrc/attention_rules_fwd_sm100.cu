@@ -197,7 +197,7 @@ rules_fwd_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const int q0 = (n_q - 1 - (int)(blockIdx.x / groups)) * BLK;  // the longest rows of a causal mask first
   const int h = (int)(blockIdx.x % groups) % p.H, b = (int)(blockIdx.x % groups) / p.H;
   const int hkv = h / (p.H / p.Hkv);
-  const int prefix = p.prefix != nullptr ? p.prefix[b] : 0;
+  const int prefix = prefix_of(p, b);
   int first, last;  // tiles of keys
   keys_of_rows(p, q0, min(q0 + BLK, p.Tq) - 1, prefix, first, last);
   first /= BLK;

@@ -92,6 +92,13 @@ def test_rules(rule, dtype):
     _check(*_inputs(B, T, T, H, K, D, dtype), _rules(rule, B, T, H))
 
 
+@pytest.mark.parametrize("prefix", [torch.tensor([-2 ** 31, 2 ** 31 - 1, -1], dtype=torch.int32), torch.tensor([-2 ** 40, 2 ** 40, -2 ** 63])], ids=["int32", "int64"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=_names)
+def test_prefixes_at_the_ends_of_their_type(prefix, dtype):
+    """Less than none is none, more than all is all, in each direction."""
+    _check(*_inputs(3, 300, 300, 4, 2, 64, dtype), dict(prefix_lengths=prefix.cuda(), is_causal=True))
+
+
 @pytest.mark.parametrize("D", [8, 24, 64, 72, 80, 96, 120, 128, 200, 256, 7, 33])
 @pytest.mark.parametrize("dtype", DTYPES, ids=_names)
 def test_head_sizes(D, dtype):
