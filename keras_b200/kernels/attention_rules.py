@@ -252,6 +252,16 @@ class RuleAttention(torch.autograd.Function):
         return (*grads, None, None, None, None, None, None, None)
 
 
+def _savable(rules):
+    """The rules with ordinary tensors: one that was made in inference mode cannot be saved for the gradients."""
+    slopes, prefix = (t.clone() if t is not None and t.is_inference() else t for t in (rules.slopes, rules.prefix))
+    segments = rules.segments
+    if segments is not None and (segments[0].is_inference() or segments[1].is_inference()):
+        rows = segments[0].clone()
+        segments = rows, rows if segments[1] is segments[0] else segments[1].clone()
+    return rules if slopes is rules.slopes and prefix is rules.prefix and segments is rules.segments else rules._replace(slopes=slopes, prefix=prefix, segments=segments)
+
+
 def attention(q, k, v, rules, plain):
     """Attention on this package's kernels, or ``None`` when the call does not fit them.  ``plain(q, k, v, rules)``: the form that second
     derivatives go through."""
@@ -264,6 +274,7 @@ def attention(q, k, v, rules, plain):
         q, k, v = unit(q), unit(k), unit(v)
         plan = plan_of(q, k, v)
     if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        rules = _savable(rules)
         rows, keys = rules.segments or (None, None)
         return RuleAttention.apply(q, k, v, rules.slopes, rules.prefix, rows, keys, rules, plain, plan)
     return forward(q, k, v, rules, segment_ranges(rules), False, plan)[0]

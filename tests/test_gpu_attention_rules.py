@@ -302,6 +302,20 @@ def test_saved_rules_must_not_be_written_to():
         out.backward(do)
 
 
+@pytest.mark.parametrize("pair", [False, True])
+def test_rules_that_were_made_in_inference_mode(pair):
+    """A data pipeline may run in that mode: its masks do for training all the same."""
+    q, k, v, do = _inputs(3, 50, 50, 4, 2, 64, torch.bfloat16)
+    rules = dict(_rules("all", 3, 50, 4), distance_slopes=torch.tensor(_slopes(4), device="cuda"))
+    want = _run(q, k, v, do, rules)
+    with torch.inference_mode():
+        rules = {n: t.clone() if isinstance(t, torch.Tensor) else t for n, t in rules.items()}
+    assert rules["segment_ids"].is_inference() and rules["distance_slopes"].is_inference()
+    if pair:
+        rules["segment_ids"] = (rules["segment_ids"].clone(), rules["segment_ids"])
+    assert all(torch.equal(a, b) for a, b in zip(_run(q, k, v, do, rules), want))
+
+
 def test_another_stream_and_a_recorded_step():
     q, k, v, do = _inputs(2, 333, 333, 4, 2, 64, torch.bfloat16)
     rules = dict(_rules("all", 2, 333, 4), distance_slopes=torch.tensor(_slopes(4), device="cuda"))
