@@ -52,7 +52,7 @@ def unit(t):
 class Plan:
     """What a call's types, sizes and strides settle: worked out once for each and kept, as a step calls the same layers again and again."""
 
-    __slots__ = ("fits", "unit", "tensor", "tiled", "grad_strides", "code", "sizes", "out", "lse", "pitch", "strides", "_work")
+    __slots__ = ("fits", "unit", "tensor", "tiled", "grad_strides", "code", "sizes", "out", "lse", "delta", "pitch", "strides", "_work")
 
     def __init__(self, q, k, v):
         same = (q.dtype in _CODES and k.dtype == q.dtype and v.dtype == q.dtype and k.shape == v.shape and k.shape[0] == q.shape[0] and k.shape[-1] == q.shape[-1]
@@ -71,6 +71,7 @@ class Plan:
         self.sizes = (B, H, K, T, S, D)
         self.out, self.pitch = (B, T, H, D), (T + 127) // 128 * 128
         self.lse = (B, H, self.pitch)
+        self.delta = B * H * self.pitch + (B * (H + K) if self.tensor and q.dtype == torch.float16 else 0)  # float16 keeps norms behind the sums
         self.strides = strides(q, k, v)
         o = (0 if T == 1 else H * D, 0 if H == 1 else D, 0 if B == 1 else T * H * D)
         self.grad_strides = (ctypes.c_longlong * 12)(*self.strides, *o)  # with a contiguous gradient of the result
@@ -206,7 +207,7 @@ def backward(q, k, v, out, lo, lse, grad_out, rules, ranges, want_q, want_kv):
             q, k, v, grad_out = _tiles(q), _tiles(k), _tiles(v), _tiles(grad_out)
         a, b, c, d = q.data_ptr(), k.data_ptr(), v.data_ptr(), grad_out.data_ptr()
         layout = strides(q, k, v, grad_out)
-    delta = torch.empty_like(lse)
+    delta = lse.new_empty(plan.delta)
     dq = q.new_empty(plan.out) if want_q else None
     dk = dv = work = None
     floats = 0

@@ -30,7 +30,66 @@ using namespace kbrules;
 struct Sums {
   const float *lse, *delta;  // [B, H, pitch], pitch a multiple of 128; rows beyond Tq hold +inf and 0
   int pitch;
+  const float* peaks;  // float16: [B, H] largest squared norm of a row of dO, then [B, Hkv] of V
 };
+
+// dS in float16.  |dS_ij| <= |dP_ij - delta_i| <= 2 max |dO| max |V| (norms of rows; delta is a mean of dP), but with gradients of a mean loss most dS lie far below
+// 2^-14, where float16 loses bits and then the value.  So dS goes to its products times the power of two that brings this bound to between 2^14 and 2^15, one of
+// a sequence and head (for dK of a key head), and their float32 sums are multiplied with its inverse: exact both ways, as is a gradient that comes
+// 2^n times as large or small.  With dO of size 1e-4 at 1 x 4096 x 64 dk was 8.6 times as far off as its own rounding without it, 1.2 times with it.
+// bfloat16 has float32's range and needs none.
+// Exponent of that power for squares of the norms: 2^x * 2 sqrt(g2 v2) <= 2^15; none where a gradient or the values are zero.
+__device__ __forceinline__ int room_of(float g2, float v2) {
+  const float square = g2 * v2;  // 7e-15 .. 6e11 each where they are not zero
+  return square > 0.f ? 14 - ((((__float_as_int(square) >> 23) & 255) - 127 + 2) >> 1) : 0;
+}
+__device__ __forceinline__ float power_of_two(int x) { return __int_as_float((x + 127) << 23); }
+
+// Largest squared norm of a row, a block a part of the rows of one sequence and head; rows that are not finite have no say (what they reach is
+// NaN whatever the factor).  First the blocks of x, then those of y.  A maximum does not depend on the order of its atomics.  Bound by the bytes of both.
+constexpr int PEAK_ROWS = 256;
+template <int G>
+__global__ void __launch_bounds__(256) peaks_kernel(const __half* x, Strides xs, int T, int H, const __half* y, Strides ys, int Ty, int Hy, float* peaks, int B, int D) {
+  const int parts = (T + PEAK_ROWS - 1) / PEAK_ROWS;
+  const long long first = (long long)B * H * parts;
+  long long at = blockIdx.x;
+  int each = parts, heads = H;
+  if (at >= first) {
+    at -= first;
+    peaks += (long long)B * H;
+    x = y;
+    xs = ys;
+    T = Ty;
+    heads = Hy;
+    each = (Ty + PEAK_ROWS - 1) / PEAK_ROWS;
+  }
+  const long long unit = at / each;
+  const int t0 = (int)(at % each) * PEAK_ROWS, h = (int)(unit % heads), d = (int)(threadIdx.x % G) * 8;
+  const __half* from = x + unit / heads * xs.b + h * xs.h + d;
+  float top = 0.f;
+#pragma unroll 4
+  for (int r = threadIdx.x / G; r < PEAK_ROWS; r += 256 / G) {
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (t0 + r < T && d < D) w = *reinterpret_cast<const uint4*>(from + (long long)(t0 + r) * xs.t);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float v = __half2float(reinterpret_cast<const __half*>(&w)[i]);
+      sum = fmaf(v, v, sum);
+    }
+#pragma unroll
+    for (int n = 1; n < G; n <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, n);
+    if (sum <= 3e38f) top = fmaxf(top, sum);
+  }
+  top = warp_max(top);
+  if ((threadIdx.x & 31) == 0 && top > 0.f) atomicMax(reinterpret_cast<int*>(peaks) + unit, __float_as_int(top));  // of floats without a sign, as whole numbers
+}
+void launch_peaks(const __half* g, const Strides& gs, const __half* v, const Strides& vs, float* peaks, const Rules& p, cudaStream_t stream) {
+  cudaMemsetAsync(peaks, 0, (size_t)p.B * (p.H + p.Hkv) * sizeof(float), stream);
+  const long long blocks = (long long)p.B * (p.H * (long long)((p.Tq + PEAK_ROWS - 1) / PEAK_ROWS) + p.Hkv * (long long)((p.Tk + PEAK_ROWS - 1) / PEAK_ROWS));
+  if (p.D <= 64) peaks_kernel<8><<<(unsigned)blocks, 256, 0, stream>>>(g, gs, p.Tq, p.H, v, vs, p.Tk, p.Hkv, peaks, p.B, p.D);
+  else peaks_kernel<16><<<(unsigned)blocks, 256, 0, stream>>>(g, gs, p.Tq, p.H, v, vs, p.Tk, p.Hkv, peaks, p.B, p.D);
+}
 
 // From 32 raw scores (columns e of a lane) to probabilities x and w = P (1 - tanh^2).  `from` - e is the distance of the pair; minus_lse(e): of
 // columns e and e + 1.
@@ -75,8 +134,8 @@ struct Parts {
   float* sums;  // [dk, dv][count][B, Tk, Hkv, D]
 };
 
-// 32 columns of a row in float32, or zeros.
-__device__ __forceinline__ void store_sums(float* to, uint32_t tmem, int col, int D, bool valid, bool zero) {
+// 32 columns of a row in float32 times a power of two, or zeros.
+__device__ __forceinline__ void store_sums(float* to, uint32_t tmem, int col, int D, float factor, bool valid, bool zero) {
   float o[32];
   if (!zero) {
     tmem_ld32(tmem, reinterpret_cast<uint32_t*>(o));
@@ -85,7 +144,7 @@ __device__ __forceinline__ void store_sums(float* to, uint32_t tmem, int col, in
 #pragma unroll
   for (int u = 0; u < 8; ++u)
     if (valid && col + u * 4 < D)
-      *reinterpret_cast<float4*>(to + col + u * 4) = zero ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[u * 4], o[u * 4 + 1], o[u * 4 + 2], o[u * 4 + 3]);
+      *reinterpret_cast<float4*>(to + col + u * 4) = zero ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o[u * 4] * factor, o[u * 4 + 1] * factor, o[u * 4 + 2] * factor, o[u * 4 + 3] * factor);
 }
 
 // dk and dv from the sums of their parts, in order.
@@ -140,6 +199,7 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 const __grid_constant__ CUtensorMap map_g, const Rules p, const Cap c_, const Sums sums, T* dk, T* dv, const Parts parts, int* err) {
   using C = DkvCfg<D>;
   constexpr int TILE = C::TILE, ST = C::STAGES;
+  constexpr bool RANGE = __is_same(T, __half);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t base = smem_u32(smem_raw);
   if (base & 1023u) {
@@ -220,6 +280,13 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     rows_of_keys(p, key, key, prefix, lo, hi);
     if (key >= p.Tk) hi = -1;
     if (p.seg_k != nullptr) own = key < p.Tk ? p.seg_k[(long long)b * p.Tk + key] : -1;
+    int room = 0;  // dS is worked with times 2^room
+    if constexpr (RANGE) {
+      float peak = 0.f;
+      for (int h = 0; h < group; ++h) peak = fmaxf(peak, sums.peaks[b * p.H + hkv * group + h]);
+      room = room_of(peak, sums.peaks[p.B * p.H + b * p.Hkv + hkv]);
+    }
+    const float up = power_of_two(room), down = power_of_two(-room);
     bool ok = true;
     int it = 0, g = g0, n = n0;
     Score f = score_of(p, hkv * group + g);
@@ -256,8 +323,10 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           const uint64_t delta2 = *reinterpret_cast<const uint64_t*>(lse + 128 + e);
+          const uint64_t dp2 = pack_f32x2(x[e], x[e + 1]);
+          const uint64_t past2 = RANGE ? fma_f32x2(delta2, both(-up), mul_f32x2(dp2, both(up))) : fma_f32x2(delta2, both(-1.f), dp2);
           float d0, d1;
-          unpack_f32x2(mul_f32x2(fma_f32x2(delta2, both(-1.f), pack_f32x2(x[e], x[e + 1])), pack_f32x2(w[e], w[e + 1])), d0, d1);
+          unpack_f32x2(mul_f32x2(past2, pack_f32x2(w[e], w[e + 1])), d0, d1);
           packed[e / 2] = pack_16<T>(d0, d1);
         }
         tmem_st16(tP + at, packed);
@@ -280,12 +349,12 @@ rules_dkv_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       float* to = parts.sums + (quarter < 2 ? (long long)parts.count * size : 0) + part * size + row;
 #pragma unroll 1
       for (int c = (quarter & 1) * (D / 2); c < ((quarter & 1) + 1) * (D / 2); c += 32)
-        store_sums(to, (quarter < 2 ? tV : tK) + lane_base + (uint32_t)c, c, p.D, key < p.Tk, mine == 0);
+        store_sums(to, (quarter < 2 ? tV : tK) + lane_base + (uint32_t)c, c, p.D, quarter < 2 ? 1.f : down, key < p.Tk, mine == 0);
     } else if (ok) {  // half of the warps store dV, the others dK, each half of the columns
       T* to = (quarter < 2 ? dv : dk) + (((long long)b * p.Tk + min(key, p.Tk - 1)) * p.Hkv + hkv) * p.D;
 #pragma unroll 1
       for (int c = (quarter & 1) * (D / 2); c < ((quarter & 1) + 1) * (D / 2); c += 32)
-        store_row(to, (quarter < 2 ? tV : tK) + lane_base + (uint32_t)c, c, p.D, quarter < 2 ? 1.f : p.scale, key < p.Tk, it == 0);
+        store_row(to, (quarter < 2 ? tV : tK) + lane_base + (uint32_t)c, c, p.D, quarter < 2 ? 1.f : p.scale * down, key < p.Tk, it == 0);
     } else {
       if (lane == 0 && err) atomicExch(err, 53);
       *abort_flag = 1;
@@ -410,6 +479,7 @@ rules_dq_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                const __grid_constant__ CUtensorMap map_g, const Rules p, const Cap c_, const Sums sums, T* dq, int* err) {
   using C = DqCfg<D>;
   constexpr int TILE = C::TILE, KS = C::KS, VS = C::VS;
+  constexpr bool RANGE = __is_same(T, __half);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t base = smem_u32(smem_raw);
   if (base & 1023u) {
@@ -483,7 +553,9 @@ rules_dq_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     if (qi >= p.Tq) hi = -1;
     if (p.seg_q != nullptr) own = qi < p.Tq ? p.seg_q[(long long)b * p.Tq + qi] : -1;
     const long long sum_at = ((long long)b * p.H + h) * sums.pitch + qi;
-    const uint64_t minus_lse2 = both(-sums.lse[sum_at]), minus_delta2 = both(-sums.delta[sum_at]);
+    const int room = RANGE ? room_of(sums.peaks[b * p.H + h], sums.peaks[p.B * p.H + b * p.Hkv + hkv]) : 0;  // dS is worked with times 2^room
+    const float up = power_of_two(room), down = power_of_two(-room);
+    const uint64_t minus_lse2 = both(-sums.lse[sum_at]), minus_delta2 = both(-sums.delta[sum_at] * up), up2 = both(up);
     bool ok = true;
     int it = 0;
     for (int n = start; n < end; n = next(n), ++it) {
@@ -511,7 +583,8 @@ rules_dq_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 #pragma unroll
       for (int e = 0; e < 32; e += 2) {
         float d0, d1;
-        unpack_f32x2(mul_f32x2(add_f32x2(pack_f32x2(x[e], x[e + 1]), minus_delta2), pack_f32x2(w[e], w[e + 1])), d0, d1);
+        const uint64_t dp2 = pack_f32x2(x[e], x[e + 1]);
+        unpack_f32x2(mul_f32x2(RANGE ? fma_f32x2(dp2, up2, minus_delta2) : add_f32x2(dp2, minus_delta2), pack_f32x2(w[e], w[e + 1])), d0, d1);
         packed[e / 2] = pack_16<T>(d0, d1);
       }
       tmem_st16(tS, packed);
@@ -526,7 +599,7 @@ rules_dq_sm100(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     }
     if (ok) {  // a quarter of the warps for every 32 columns
       T* to = dq + (((long long)b * p.Tq + min(qi, p.Tq - 1)) * p.H + h) * p.D;
-      if (part * 32 < D) store_row(to, tQ + lane_base + (uint32_t)(part * 32), part * 32, p.D, p.scale, qi < p.Tq, it == 0);
+      if (part * 32 < D) store_row(to, tQ + lane_base + (uint32_t)(part * 32), part * 32, p.D, p.scale * down, qi < p.Tq, it == 0);
     } else {
       if (lane == 0 && err) atomicExch(err, 63);
       *abort_flag = 1;
@@ -677,9 +750,10 @@ KB_API long long kb200_attention_rules_bwd_work(int B, int H, int Hkv, int Tq, i
 }
 
 // As kb200_attention_rules_bwd for what kb200_attention_rules_fwd_sm100 takes, at most 1048576 rows and keys; lse and delta with rows `pitch` apart, a
-// multiple of 128.  work: `floats` of them, 16-byte aligned, as many as kb200_attention_rules_bwd_work says, or null.
+// multiple of 128.  peaks: float16 B * (H + Hkv) floats of workspace, bfloat16 null.  work: `floats` of them, 16-byte aligned, as many as
+// kb200_attention_rules_bwd_work says, or null.
 KB_API int kb200_attention_rules_bwd_sm100(const void* q, const void* k, const void* v, const void* grad_out, const long long* strides, const float* lse, const float* delta,
-                                           int pitch, void* dq, void* dk, void* dv, int dtype, int B, int H, int Hkv, int Tq, int Tk, int D, int* err, float* work, long long floats, float scale, float cap,
+                                           int pitch, float* peaks, void* dq, void* dk, void* dv, int dtype, int B, int H, int Hkv, int Tq, int Tk, int D, int* err, float* work, long long floats, float scale, float cap,
                                            const float* slopes, int causal, int window, const int* prefix, const int* seg_q, const int* seg_k, const void* range_q,
                                            const void* range_k, cudaStream_t stream) {
   const Rules p{B, H, Hkv, Tq, Tk, D, scale, cap, slopes, causal, window, prefix, seg_q, seg_k, (const int4*)range_q, (const int4*)range_k};
@@ -695,13 +769,18 @@ KB_API int kb200_attention_rules_bwd_sm100(const void* q, const void* k, const v
     return -2;
   }
   const bool half = dtype == 2;
+  if (half && peaks == nullptr) {
+    kb200_set_error("attention_rules_bwd_sm100: float16 needs a workspace for its rows' norms");
+    return -2;
+  }
   CUtensorMap m[4];
   if (!rules_map(&m[0], q, D, Tq, H, B, qs, 128, half) || !rules_map(&m[1], k, D, Tk, Hkv, B, ks, 128, half) || !rules_map(&m[2], v, D, Tk, Hkv, B, vs, 128, half) ||
       !rules_map(&m[3], grad_out, D, Tq, H, B, gs, 128, half)) {
     kb200_set_error("attention_rules_bwd_sm100: cuTensorMapEncodeTiled failed");
     return -3;
   }
-  const Sums sums{lse, delta, pitch};
+  const Sums sums{lse, delta, pitch, peaks};
+  if (half) launch_peaks((const __half*)grad_out, gs, (const __half*)v, vs, peaks, p, stream);
   Parts parts{parts_of(B, H, Hkv, Tq, Tk), work};
   if (work == nullptr || 2ll * parts.count * B * Tk * Hkv * D > floats) parts.count = 1;
   int rc;
@@ -715,13 +794,14 @@ KB_API int kb200_attention_rules_bwd_sm100(const void* q, const void* k, const v
 KB_API int kb200_attention_rules_delta(const void* o, const void* lo, const void* grad_out, const long long* strides, float* delta, int pitch, int dtype, int B, int H, int Tq, int D,
                                        cudaStream_t stream);
 
-// All of a gradient in one call: delta, from o, lo (may be null) and grad_out, then the above.
+// All of a gradient in one call: delta, from o, lo (may be null) and grad_out, then the above.  delta: B * H * pitch floats, and float16 B * (H + Hkv) more
+// behind them for the norms.
 KB_API int kb200_attention_rules_grads_sm100(const void* q, const void* k, const void* v, const void* o, const void* lo, const void* grad_out, const long long* strides,
                                              const float* lse, float* delta, int pitch, void* dq, void* dk, void* dv, int dtype, int B, int H, int Hkv, int Tq, int Tk, int D, int* err,
                                              float* work, long long floats, float scale, float cap, const float* slopes, int causal, int window, const int* prefix, const int* seg_q, const int* seg_k,
                                              const void* range_q, const void* range_k, cudaStream_t stream) {
   const int rc = kb200_attention_rules_delta(o, lo, grad_out, strides + 9, delta, pitch, dtype, B, H, Tq, D, stream);
   return rc != 0 ? rc
-                 : kb200_attention_rules_bwd_sm100(q, k, v, grad_out, strides, lse, delta, pitch, dq, dk, dv, dtype, B, H, Hkv, Tq, Tk, D, err, work, floats, scale, cap, slopes, causal, window, prefix,
+                 : kb200_attention_rules_bwd_sm100(q, k, v, grad_out, strides, lse, delta, pitch, dtype == 2 ? delta + (long long)B * H * pitch : nullptr, dq, dk, dv, dtype, B, H, Hkv, Tq, Tk, D, err, work, floats, scale, cap, slopes, causal, window, prefix,
                                                    seg_q, seg_k, range_q, range_k, stream);
 }

@@ -201,6 +201,59 @@ def test_saved_tensors_that_come_back_in_another_layout(dtype):
         assert torch.equal(a, b)
 
 
+def _gradients(q, k, v, do, rules):
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    return torch.autograd.grad(keras.ops.dot_product_attention(*leaves, **rules), leaves, do)
+
+
+@pytest.mark.parametrize("B,T,H,K,D", [(2, 300, 4, 4, 64), (1, 900, 8, 1, 128), (2, 200, 4, 2, 80)])
+@pytest.mark.parametrize("cap", [None, 50.0])
+def test_float16_gradients_keep_their_bits_at_every_size(B, T, H, K, D, cap):
+    """A gradient of the result that is 2^16 times as small gives gradients that are, bit for bit, wherever those are still normal numbers.  (Its values are multiples of
+    2^-14, so that it is exact itself and its numbers are normal too: of others the tensor cores' sums may be cut off elsewhere.)"""
+    q, k, v, _ = _inputs(B, T, T, H, K, D, torch.float16)
+    v = v * 64
+    do = torch.randint(-8, 9, q.shape, generator=torch.Generator().manual_seed(1)).cuda().half() * 4
+    rules = dict(is_causal=True, sliding_window=T, attn_logits_soft_cap=cap)
+    for name, large, small in zip(("dq", "dk", "dv"), _gradients(q, k, v, do, rules), _gradients(q, k, v, do * 2.0 ** -16, rules)):
+        assert torch.isfinite(large).all()
+        normal = small.abs() > 2.0 ** -14  # 2^-14 itself is also what the numbers of half a step below it are rounded to
+        assert name == "dv" or normal.float().mean() > 0.5
+        assert torch.equal(small.double()[normal] * 2 ** 16, large.double()[normal]), name
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T", [300, 1024])
+def test_float16_gradients_of_a_mean_loss(T, D):
+    """As far off as two roundings, not as what float16 leaves of numbers far below 2^-14.  An element is rounded once, with an error of root mean square r; dS was
+    rounded before its sum, an independent error of the same relative size in each term, whose sum is r again where the terms do not cancel, half as much more
+    where they do (1.5 r in 64 bits with that rounding alone, one in all by root sum): 2 r bounds it.  The sequences' gradients differ by 10^4."""
+    q, k, v, do = _inputs(2, T, T, 2, 2, D, torch.float16, q_scale=3.0)
+    do = (do.float() * torch.tensor([1.0, 1e-4], device="cuda").view(2, 1, 1, 1)).half()
+    rules = dict(is_causal=True, sliding_window=T)
+    found = _definition(q, k, v, do, rules)
+    for name, got in zip(("dq", "dk"), _gradients(q, k, v, do, rules)):
+        exact = found[name][0]
+        for b in range(2):
+            rounding = (exact[b].half().double() - exact[b]).square().mean().sqrt()
+            off = (got[b].double().cpu() - exact[b]).square().mean().sqrt()
+            assert off <= 2 * rounding, (name, b, float(off / rounding))
+
+
+def test_float16_gradients_beside_infinite_and_zero_ones():
+    """What is infinite in one sequence, and zero in another, has no say in a third."""
+    q, k, v, do = _inputs(3, 260, 260, 2, 1, 64, torch.float16)
+    rules = dict(is_causal=True, sliding_window=100)
+    want = _gradients(q, k, v, do, rules)
+    do[0, 40, 1, 3], do[1] = float("inf"), 0
+    v[0, 7] = float("nan")
+    got = _gradients(q, k, v, do, rules)
+    for a, b in zip(got, want):
+        assert torch.equal(a[2], b[2]) and not a[1].any()
+    v[2] = 0
+    assert not _gradients(q, k, v, do, rules)[0][2].any()
+
+
 def _turned(t):
     """The same values, with the first and the last dimension's places in memory exchanged."""
     return t.transpose(0, -1).contiguous().transpose(0, -1) if t.ndim > 1 else torch.stack([t, t], 1)[:, 0]
