@@ -14,6 +14,7 @@ from keras_b200.kernels import dispatch
 
 Rules = kernel_rules.Rules
 _INT32 = torch.iinfo(torch.int32)
+_WIDE = (torch.int64, torch.uint32)
 
 
 def _refuse(text):
@@ -50,28 +51,44 @@ def slopes(value, heads, device):
     return value.to(torch.float32).contiguous()
 
 
-def _whole(value, name, shape, device):
-    """An integer tensor of that shape as int32; what does not fit is held at the type's ends."""
+def _integers(value, name, shape, device):
+    """An integer tensor of that shape on that device."""
     value = convert_to_tensor(value) if not isinstance(value, torch.Tensor) else value
-    if value.dtype.is_floating_point or value.dtype.is_complex or value.dtype == torch.bool:
+    if value.dtype.is_floating_point or value.dtype.is_complex or value.dtype in (torch.bool, torch.uint64):
         _refuse(f"`{name}` has to be of an integer type. Received: {value.dtype}")
     if tuple(value.shape) != shape:
         _refuse(f"`{name}` has to have the shape {shape}. Received: {tuple(value.shape)}")
     if value.device != device:
         value = value.to(device) if value.device.type == "cpu" else _refuse(f"`{name}` has to be on the device of the query. Received: {value.device} and {device}")
-    if value.dtype != torch.int32:
-        value = value.clamp(_INT32.min, _INT32.max).to(torch.int32) if value.dtype == torch.int64 else value.to(torch.int32)
-    return value.contiguous()
+    return value
+
+
+def _whole(value, name, shape, device):
+    """The same as int32; what does not fit is held at the type's ends."""
+    value = _integers(value, name, shape, device)
+    if value.dtype in _WIDE:
+        value = value.to(torch.int64).clamp(_INT32.min, _INT32.max)
+    return value.to(torch.int32).contiguous()
+
+
+def _ids(*tensors):
+    """Segment ids as int32.  Wider ones may differ in bits that int32 has no place for (a document's hash): they become their places in the order of a
+    sequence's ids, which are equal where the ids are."""
+    if not any(t.dtype in _WIDE for t in tensors):
+        return tuple(t.to(torch.int32).contiguous() for t in tensors)
+    tensors = [t.to(torch.int64).contiguous() for t in tensors]
+    order = torch.cat(tensors, dim=1).sort(dim=1).values if len(tensors) > 1 else tensors[0].sort(dim=1).values
+    return tuple(torch.searchsorted(order, t, out_int32=True).masked_fill_(t < 0, -1) for t in tensors)
 
 
 def segments(value, B, T, S, device):
     if isinstance(value, tuple):
         if len(value) != 2:
             _refuse("`segment_ids` has to be one tensor, or a tuple of those of the rows and of the keys.")
-        return _whole(value[0], "segment_ids", (B, T), device), _whole(value[1], "segment_ids", (B, S), device)
+        return _ids(_integers(value[0], "segment_ids", (B, T), device), _integers(value[1], "segment_ids", (B, S), device))
     if T != S:
         _refuse("`segment_ids` has to be a tuple of those of the rows and of the keys where their lengths differ.")
-    value = _whole(value, "segment_ids", (B, T), device)
+    value, = _ids(_integers(value, "segment_ids", (B, T), device))
     return value, value
 
 

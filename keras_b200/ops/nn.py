@@ -705,7 +705,8 @@ def dot_product_attention(query, key, value, bias=None, mask=None, scale=None, i
       into a CUDA graph they have to be a tensor on the device.
     * ``sliding_window``: row i sees the keys with ``|i - j| < sliding_window``.
     * ``segment_ids``: int32 ``[B, T]``, or a tuple of those of the rows ``[B, T]`` and of the keys ``[B, S]``.  Rows see the keys of their own segment; a negative
-      id is padding, which sees nothing and is seen by nobody.  Ids may come in any order; tiles without a common id are left out.
+      id is padding, which sees nothing and is seen by nobody.  Ids may come in any order; tiles without a common id are left out.  (Ids of 64 bits are
+      compared as such: each call sorts them first.)
     * ``prefix_lengths``: int32 ``[B]``, with ``is_causal``: the first keys of each sequence, as many as that, are seen by every row.
 
     With any of the four, a row that sees nothing is zero and has no gradient (a fully masked row of ``mask`` alone attends uniformly).  Values

@@ -69,6 +69,31 @@ def test_rows_and_keys_of_different_lengths_and_rows_that_see_nothing():
     assert not grads[1][1].any()
 
 
+def wide_ids():
+    """Ids that int32 does not tell apart, and what they stand for."""
+    small = torch.tensor([[0, 0, 0, 1, 1, 2, 2, 0, -1], [3, 1, 3, 1, 3, 1, 3, 1, 3], [0, 1, 2, -1, 4, 5, 6, 7, 8]])
+    return {"hashes": torch.where(small < 0, small, small * 2 ** 33 + 2 ** 40 + 5), "padding": torch.where(small < 0, -2 ** 50 + small, 2 ** 62 - small),
+            "uint32": torch.where(small < 0, torch.arange(27).reshape(3, 9) + 100, small + 2 ** 31 + 3).to(torch.uint32)}, small
+
+
+@pytest.mark.parametrize("name", ["hashes", "padding", "uint32"])
+@pytest.mark.parametrize("pair", [False, True])
+def test_segment_ids_beyond_int32(name, pair):
+    wide, small = wide_ids()
+    if name == "uint32":  # has no padding: an id of its own in its place, which sees itself
+        small = torch.where(small < 0, torch.arange(27).reshape(3, 9) + 100, small)
+    q, k, v, do = _inputs(3, 9, 9, 4, 2, 8)
+    given = (wide[name], wide[name].clone()) if pair else wide[name]
+    found = _definition(q, k, v, do, dict(segment_ids=small))
+    definition.check("out", keras.ops.dot_product_attention(q, k, v, segment_ids=given), found)
+
+
+def test_segment_ids_of_64_bits_that_may_be_none_are_refused():
+    q, k, v, _ = _inputs(1, 9, 9, 4, 2, 8)
+    with pytest.raises(ValueError, match="integer type"):
+        keras.ops.dot_product_attention(q, k, v, segment_ids=torch.zeros(1, 9, dtype=torch.uint64))
+
+
 def test_gradients_agree_with_differences():
     g = torch.Generator().manual_seed(3)
     leaves = [torch.randn(1, 6, h, 4, generator=g, dtype=torch.float64, requires_grad=True) for h in (4, 2, 2)]

@@ -99,6 +99,22 @@ def test_prefixes_at_the_ends_of_their_type(prefix, dtype):
     _check(*_inputs(3, 300, 300, 4, 2, 64, dtype), dict(prefix_lengths=prefix.cuda(), is_causal=True))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=_names)
+def test_segment_ids_beyond_int32(dtype):
+    """Rows and keys of their own lengths, in no order, and in a recorded step."""
+    rows, keys = _ids(2, 150, "mixed"), _ids(2, 260, "mixed")
+    args, small = _inputs(2, 150, 260, 4, 2, 64, dtype), (rows, keys)
+    wide = tuple(torch.where(t < 0, -2 ** 40 + t, 2 ** 40 + t.long() * 2 ** 34) for t in small)
+    want = _run(*args, dict(segment_ids=small))
+    assert all(torch.equal(a, b) for a, b in zip(_run(*args, dict(segment_ids=wide)), want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = keras.ops.dot_product_attention(*args[:3], segment_ids=wide)
+    graph.replay()
+    assert torch.equal(out, want[4])
+    del graph
+
+
 @pytest.mark.parametrize("D", [8, 24, 64, 72, 80, 96, 120, 128, 200, 256, 7, 33])
 @pytest.mark.parametrize("dtype", DTYPES, ids=_names)
 def test_head_sizes(D, dtype):
