@@ -99,6 +99,33 @@ def plan_of(q, k, v):
     return plan
 
 
+_SMALL = 5 << 18  # pairs of rows and keys, over all heads
+
+
+def cap_pays(q, k, v, causal):
+    """Whether a call whose only rule is a cap is faster on these kernels than in the library's operations over whole score matrices.  On the tensor cores always
+    (2 to 20 times).  The FMA kernels are bound by their arithmetic, with nothing but a causal mask to leave out, where the library multiplies
+    at twice to fifty times their rate and pays for some ten passes over the matrix.  Measured, as multiples of the library's speed:
+
+    * up to 1.3 million pairs, where the library's launches last longer than either: 1.0 to 5 (1 x 64 x 8 x 256 float32 forward 43 us against 84)
+    * fewer than 128 tiles of 64 rows, which leave SMs without a block: from 0.3 (1 x 1024 x 4 x 64 float32 forward 0.6)
+    * heads of up to 64: forward 1.0 to 1.6, causal 1.4 to 3.5; trained 0.6 to 0.85, causal 1.1 to 1.9
+    * up to 128: forward 0.4 to 0.95, causal 1.1 to 2.2; trained 0.3 to 0.85, causal 1.0 to 1.3 in float32 and 0.6 to 0.7 in 16 bits
+    * beyond: forward 0.2 to 0.9, causal 1.1 to 1.45 in float32 (0.85 to 0.95 with 128 tiles) and 0.6 to 0.8 in 16 bits; trained 0.1 to 0.7
+    """
+    (B, T, H, D), S, narrow = q.shape, k.shape[1], q.dtype != torch.float32
+    if (narrow and D <= 128 and D % 8 == 0) or B * H * T * S <= _SMALL:
+        return True
+    tiles = B * H * ((T + 63) // 64)
+    if tiles < 128:
+        return False
+    training = (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled()
+    halved = causal and min(T, S) >= 256  # of one or two tiles a causal mask leaves out nothing
+    if D <= 64:
+        return halved or not training or max(T, S) <= 128
+    return halved and ((D <= 128 and not (narrow and training)) or (tiles >= 148 and not narrow and not training))
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 

@@ -695,7 +695,8 @@ def dot_product_attention(query, key, value, bias=None, mask=None, scale=None, i
                           distance_slopes=None, sliding_window=None, segment_ids=None, prefix_lengths=None, cache=None):
     """Inputs are ``[B, T, N, H]`` / ``[B, S, K, H]`` (K divides N: grouped-query).
 
-    ``attn_logits_soft_cap``: scores become ``cap * tanh(score / cap)``.
+    ``attn_logits_soft_cap``: scores become ``cap * tanh(score / cap)``.  By itself it runs in the library's operations wherever those are faster
+    than this package's kernels (large float32 products that no mask halves, wide heads).
 
     Rules about who sees whom, and a bias by distance, take the place of ``[T, S]`` masks and biases and can be combined with each other, with the cap
     and with ``is_causal``.  Both directions run on this package's kernels for float32, bfloat16 and float16 heads of up to 256; together with

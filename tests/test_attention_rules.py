@@ -412,3 +412,14 @@ def _trains_after(kind, how, path):
 def test_slopes_of_a_transform_do_not_outlive_it(kind, how, tmp_path):
     """A layer that is first called under an export, a function transform, a trace or in inference mode trains as one that was not."""
     _trains_after(kind, how, tmp_path)
+
+
+def test_an_exported_cap_takes_any_batch(tmp_path):
+    """Which way a call takes goes by its sizes, and says nothing of those of an export."""
+    x = keras.Input((8, 4, 16))
+    model = keras.Model(x, keras.layers.Lambda(lambda t: keras.ops.dot_product_attention(t, t, t, attn_logits_soft_cap=3.0))(x))
+    model.export(str(tmp_path / "m"), format="torch_export", verbose=False)
+    program = torch.export.load(str(tmp_path / "m" / "serve.pt2")).module()
+    for n in (1, 3, 6000):
+        t = torch.randn(n, 8, 4, 16, generator=torch.Generator().manual_seed(n))
+        torch.testing.assert_close(program(t), keras.ops.dot_product_attention(t, t, t, attn_logits_soft_cap=3.0))

@@ -270,6 +270,39 @@ def test_float16_gradients_beside_infinite_and_zero_ones():
     assert not _gradients(q, k, v, do, rules)[0][2].any()
 
 
+@pytest.mark.parametrize("B,T,H,D,dtype,causal,forward,trained", [
+    (2, 1024, 8, 64, torch.bfloat16, False, True, True), (2, 1024, 8, 128, torch.float16, True, True, True), (1, 64, 8, 256, torch.bfloat16, False, True, True),
+    (1, 1024, 4, 64, torch.float32, True, False, False), (2, 1024, 8, 64, torch.float32, False, True, False), (2, 1024, 8, 64, torch.float32, True, True, True),
+    (64, 64, 16, 64, torch.float32, False, True, True), (64, 64, 16, 128, torch.float32, True, False, False),
+    (2, 1024, 8, 128, torch.float32, False, False, False), (2, 1024, 8, 128, torch.float32, True, True, True), (2, 1024, 8, 100, torch.bfloat16, True, True, False),
+    (2, 1024, 8, 256, torch.float32, True, True, False), (2, 1024, 8, 256, torch.bfloat16, True, False, False), (2, 1024, 8, 160, torch.float16, False, False, False),
+], ids=str)
+def test_a_cap_alone_runs_where_it_is_faster(B, T, H, D, dtype, causal, forward, trained, monkeypatch):
+    """The library's operations took such calls before there were kernels: where those are faster they still do."""
+    q, k, v, do = _inputs(B, T, T, H, H, D, dtype)
+    calls = _spy(monkeypatch)
+    with torch.no_grad():
+        out = keras.ops.dot_product_attention(q, k, v, is_causal=causal, attn_logits_soft_cap=20.0)
+    assert bool(calls["forward"]) == forward
+    calls["forward"] = 0
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    again = keras.ops.dot_product_attention(*leaves, is_causal=causal, attn_logits_soft_cap=20.0)
+    grads = torch.autograd.grad(again, leaves, do)
+    assert bool(calls["forward"]) == bool(calls["backward"]) == trained
+    assert out.shape == again.shape == q.shape and out.dtype == dtype and all(torch.isfinite(t).all() for t in (out, again, *grads))
+
+
+def _spy(monkeypatch):
+    """How often the kernels' two directions run from here on."""
+    calls = {"forward": 0, "backward": 0}
+    for name in calls:
+        def spied(*a, _name=name, _fn=getattr(attention_rules, name), **k):
+            calls[_name] += 1
+            return _fn(*a, **k)
+        monkeypatch.setattr(attention_rules, name, spied)
+    return calls
+
+
 def _turned(t):
     """The same values, with the first and the last dimension's places in memory exchanged."""
     return t.transpose(0, -1).contiguous().transpose(0, -1) if t.ndim > 1 else torch.stack([t, t], 1)[:, 0]
@@ -432,17 +465,6 @@ def test_shared_key_heads_under_a_trace(rules):
     traced = torch.jit.trace(lambda *t: keras.ops.dot_product_attention(*t, is_causal=True, **rules), (q, k, v), check_trace=False)
     want = _definition(q, k, v, None, dict(rules, is_causal=True))
     definition.check("out", traced(q, k, v), want)
-
-
-def _spy(monkeypatch):
-    """How often the kernels' two directions run from here on."""
-    calls = {"forward": 0, "backward": 0}
-    for name in calls:
-        def spied(*a, _name=name, _fn=getattr(attention_rules, name), **k):
-            calls[_name] += 1
-            return _fn(*a, **k)
-        monkeypatch.setattr(attention_rules, name, spied)
-    return calls
 
 
 @pytest.mark.parametrize("how", TRANSFORMS)
