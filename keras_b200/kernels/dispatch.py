@@ -377,15 +377,6 @@ def rule_attention(q, k, v, rules, plain):
     return attention_rules.attention(q, k, v, rules, plain)
 
 
-def capped_attention(q, k, v, rules, plain):
-    """Attention whose only rule is a cap, or ``None`` also where the library's operations are faster."""
-    if not enabled(q):
-        return None
-    from keras_b200.kernels import attention_rules
-
-    return attention_rules.attention(q, k, v, rules, plain) if attention_rules.cap_pays(q, k, v, rules.causal) else None
-
-
 def cached_attention(q, k, v, pool_k, pool_v, pages, lengths, rules):
     if not enabled(q):
         return None

@@ -173,10 +173,11 @@ def attend(q, k, v, rules, bias, mask, kernels):
 
 def capped(q, k, v, scale, is_causal, cap):
     """A call whose only rule is the cap, on the kernels, or ``None``: what they do not take, or not as fast, stays with the library's operations."""
+    if not dispatch.enabled(q) or not kernel_rules.cap_pays(q, k, v, is_causal):  # in this order: an export's sizes decide nothing
+        return None
     if isinstance(cap, (bool, torch.Tensor)) or not isinstance(cap, numbers.Real) or not 0 < cap < math.inf or isinstance(scale, torch.Tensor):
         return None
-    rules = Rules(float(scale), float(cap), None, bool(is_causal), None, None, None)
-    return dispatch.capped_attention(q, k, v, rules, plain)
+    return kernel_rules.attention(q, k, v, Rules(float(scale), float(cap), None, bool(is_causal), None, None, None), plain)
 
 
 # ------------------------------------------------------------------------------------------------ the paged cache
