@@ -7,7 +7,7 @@ import torch
 import keras_b200 as keras
 from keras_b200.kernels import attention, attention_cache, attention_rules, ops as kops
 from tests import attention_definition as definition
-from tests.test_attention_rules import SLOPES, TRANSFORMS, _Decoder, _generation, _trains_after
+from tests.test_attention_rules import SLOPES, TRANSFORMS, _Decoder, _generation, _layer, _trains_after
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
@@ -465,6 +465,33 @@ def test_shared_key_heads_under_a_trace(rules):
     traced = torch.jit.trace(lambda *t: keras.ops.dot_product_attention(*t, is_causal=True, **rules), (q, k, v), check_trace=False)
     want = _definition(q, k, v, None, dict(rules, is_causal=True))
     definition.check("out", traced(q, k, v), want)
+
+
+@pytest.mark.parametrize("kind", ["mha", "gqa"])
+@pytest.mark.parametrize("policy", ["float32", "mixed_bfloat16"])
+def test_a_layer_with_a_cap_alone_runs_on_the_kernels_in_both_directions(kind, policy, monkeypatch):
+    """Against the same weights with the kernels refused.  Sums of up to 64 products on values of size one, through three matrices: float32 some hundred roundings of
+    2^-24; bfloat16 about eight of 2^-8 each way, of the whole gradient's size."""
+    keras.config.set_dtype_policy(policy)
+    x = torch.randn(4, 64, 64, generator=torch.Generator().manual_seed(0)).cuda()
+    up = torch.randn(4, 64, 64, generator=torch.Generator().manual_seed(1)).cuda()
+    found, weights = [], None
+    for kernels in (True, False):
+        keras.utils.set_random_seed(0)
+        if not kernels:
+            keras.config.disable_flash_attention()
+        layer = _layer(kind, attn_logits_soft_cap=2.0)
+        keras.config.enable_flash_attention()
+        layer.build((4, 64, 64), (4, 64, 64))
+        weights = weights or layer.get_weights()
+        layer.set_weights(weights)
+        calls = _spy(monkeypatch)
+        out = layer(x, x, use_causal_mask=True)
+        out.float().backward(up)
+        assert calls == {"forward": int(kernels), "backward": int(kernels)}
+        found.append([out.detach().float(), *(v.value.grad.float() for v in layer.trainable_variables)])
+    for a, b in zip(*found):
+        assert (a - b).norm() <= (1e-5 if policy == "float32" else 16 * 2.0 ** -8) * b.norm()
 
 
 @pytest.mark.parametrize("how", TRANSFORMS)
