@@ -2,7 +2,7 @@
 
 ``attention`` takes query/key/value in the ``[batch, time, heads, head_dim]`` layout of the attention layers and a ``Rules``: a cap on the
 scores, a bias by distance, causal, prefix, window and segment masks.  Both directions run on this package's kernels; a gradient that is
-itself differentiated takes the plain form.
+itself differentiated, or one of a batch of them, takes the plain form.
 """
 
 import collections
@@ -254,6 +254,11 @@ def backward(q, k, v, out, lo, lse, grad_out, rules, ranges, want_q, want_kv):
     return dq, dk, dv
 
 
+def _of_a_batch(t):
+    """Whether it is many tensors in one (``is_grads_batched``, ``torch.func``), which has no address."""
+    return torch._C._functorch.is_legacy_batchedtensor(t) or torch._C._functorch.is_functorch_wrapped_tensor(t)
+
+
 class RuleAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, slopes, prefix, rows, keys, rules, plain, plan):
@@ -270,9 +275,11 @@ class RuleAttention(torch.autograd.Function):
         r = ctx.rules
         rules = Rules(r.scale, r.cap, slopes, r.causal, r.window, prefix, None if rows is None else (rows, keys))
         need = ctx.needs_input_grad
-        if torch.is_grad_enabled():  # the gradient is differentiated in its turn
+        again = torch.is_grad_enabled()  # the gradient is differentiated in its turn
+        if again or _of_a_batch(grad_out):
             wanted = [t for t, n in zip((q, k, v), need) if n]
-            given = iter(torch.autograd.grad(ctx.plain(q, k, v, rules), wanted, grad_out, create_graph=True))
+            with torch.enable_grad():
+                given = iter(torch.autograd.grad(ctx.plain(q, k, v, rules), wanted, grad_out, create_graph=again))
             grads = [next(given) if n else None for n in need[:3]]
         else:
             dq, dk, dv = backward(q, k, v, out, lo, lse, grad_out, rules, (range_q, range_k), need[0], need[1] or need[2])

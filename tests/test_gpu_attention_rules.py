@@ -394,6 +394,21 @@ def test_second_derivatives():
         torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-4)  # float32 sums of a few hundred terms of size one, squared
 
 
+@pytest.mark.parametrize("rules", [dict(attn_logits_soft_cap=5.0), dict(sliding_window=7, is_causal=True)], ids=["cap", "window"])
+def test_a_batch_of_gradients_at_once(rules):
+    """A vectorized Jacobian hands the backward pass a tensor without an address of its own."""
+    q, k, v, _ = _inputs(1, 20, 20, 2, 1, 8, torch.float32)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    out = keras.ops.dot_product_attention(*leaves, **rules)
+    batch = torch.randn(3, *out.shape, generator=torch.Generator().manual_seed(1)).cuda()
+    many = torch.autograd.grad(out, leaves, batch, is_grads_batched=True, retain_graph=True)
+    one = [torch.autograd.grad(out, leaves, g, retain_graph=True) for g in batch]
+    for i, got in enumerate(many):
+        torch.testing.assert_close(got, torch.stack([g[i] for g in one]), rtol=1e-4, atol=1e-5)  # float32 sums of twenty terms of size one, twice
+    many = torch.autograd.grad(out, leaves[:2], batch, is_grads_batched=True, create_graph=True)
+    assert many[0].requires_grad and many[1].shape == (3, *k.shape)
+
+
 def test_saved_rules_must_not_be_written_to():
     q, k, v, do = _inputs(1, 20, 20, 2, 1, 64, torch.bfloat16)
     ids = torch.zeros(1, 20, dtype=torch.int32, device="cuda")
