@@ -256,6 +256,27 @@ def test_float16_gradients_of_a_mean_loss(T, D):
             assert off <= 2 * rounding, (name, b, float(off / rounding))
 
 
+def test_float16_gradients_of_recorded_steps():
+    """Two recordings, replayed in turn with gradients of very different sizes: each finds its own largest norms again."""
+    graphs = []
+    for B, T, H, K in ((2, 200, 4, 2), (1, 300, 8, 1)):
+        q, k, v, do = _inputs(B, T, T, H, K, 64, torch.float16)
+        leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+        _gradients(q, k, v, do, dict(is_causal=True, attn_logits_soft_cap=9.0))  # a process's first launch of a kernel loads it, which no recording takes
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            made = torch.autograd.grad(keras.ops.dot_product_attention(*leaves, is_causal=True, attn_logits_soft_cap=9.0), leaves, do)
+        graphs.append((graph, leaves, do, made))
+    for factor in (1.0, 2.0 ** -10, 2.0 ** 6):
+        for graph, leaves, do, _ in graphs:
+            do.copy_(torch.randn(do.shape, generator=torch.Generator().manual_seed(3)).cuda().half() * factor)
+            graph.replay()
+        for graph, leaves, do, made in graphs:
+            want = _gradients(*(t.detach() for t in leaves), do, dict(is_causal=True, attn_logits_soft_cap=9.0))
+            assert all(torch.equal(a, b) for a, b in zip(made, want))
+    del graph, graphs
+
+
 def test_float16_gradients_beside_infinite_and_zero_ones():
     """What is infinite in one sequence, and zero in another, has no say in a third."""
     q, k, v, do = _inputs(3, 260, 260, 2, 1, 64, torch.float16)
