@@ -99,7 +99,7 @@ def plan_of(q, k, v):
     return plan
 
 
-_SMALL = 5 << 18  # pairs of rows and keys, over all heads
+_SMALL, _LARGE = 5 << 18, 1 << 30  # pairs of rows and keys, over all heads
 
 
 def cap_pays(q, k, v, causal):
@@ -107,6 +107,8 @@ def cap_pays(q, k, v, causal):
     (2 to 20 times).  The FMA kernels are bound by their arithmetic, with nothing but a causal mask to leave out, where the library multiplies
     at twice to fifty times their rate and pays for some ten passes over the matrix.  Measured, as multiples of the library's speed:
 
+    * beyond 2^30 pairs the library's matrices, of 20 bytes a pair at their peak and 8 that the gradients keep, take memory that a model has other use for:
+      the kernels, whatever the time
     * up to 1.3 million pairs, where the library's launches last longer than either: 1.0 to 5 (1 x 64 x 8 x 256 float32 forward 43 us against 84)
     * fewer than 128 tiles of 64 rows, which leave SMs without a block: from 0.3 (1 x 1024 x 4 x 64 float32 forward 0.6)
     * heads of up to 64: forward 1.0 to 1.6, causal 1.4 to 3.5; trained 0.6 to 0.85, causal 1.1 to 1.9
@@ -114,7 +116,7 @@ def cap_pays(q, k, v, causal):
     * beyond: forward 0.2 to 0.9, causal 1.1 to 1.45 in float32 (0.85 to 0.95 with 128 tiles) and 0.6 to 0.8 in 16 bits; trained 0.1 to 0.7
     """
     (B, T, H, D), S, narrow = q.shape, k.shape[1], q.dtype != torch.float32
-    if (narrow and D <= 128 and D % 8 == 0) or B * H * T * S <= _SMALL:
+    if (narrow and D <= 128 and D % 8 == 0) or not _SMALL < B * H * T * S <= _LARGE:
         return True
     tiles = B * H * ((T + 63) // 64)
     if tiles < 128:

@@ -423,3 +423,13 @@ def test_an_exported_cap_takes_any_batch(tmp_path):
     for n in (1, 3, 6000):
         t = torch.randn(n, 8, 4, 16, generator=torch.Generator().manual_seed(n))
         torch.testing.assert_close(program(t), keras.ops.dot_product_attention(t, t, t, attn_logits_soft_cap=3.0))
+
+
+@pytest.mark.parametrize("B,T,pays", [(1, 100, True), (2, 4096, False), (4, 4096, False), (5, 4096, True), (1, 100000, True)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_cap_alone_makes_no_matrices_beyond_the_memory(B, T, pays, dtype):
+    """16 heads of 256, whose training is faster in the library's operations: not for few pairs, and not beyond 2^30 of them."""
+    from keras_b200.kernels import attention_rules as kernels
+
+    q = torch.empty(B, T, 16, 256, dtype=dtype, device="meta", requires_grad=True)
+    assert kernels.cap_pays(q, q, q, False) is pays
