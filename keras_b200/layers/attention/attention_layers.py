@@ -134,6 +134,9 @@ class MultiHeadAttention(Layer):
     """``attn_logits_soft_cap`` and ``distance_slopes`` (one number a head), and in a call ``segment_ids``, ``prefix_lengths`` and ``cache``, are those of
     ``ops.dot_product_attention``; a call with a ``cache`` is causal whatever ``use_causal_mask`` says and carries no gradient.
 
+    A mask beside such rules, one that an input carries from ``Embedding(mask_zero=True)`` among them, makes a ``[batch, heads, time, time]`` matrix; padding
+    that is given as negative ``segment_ids`` makes none.
+
     The pools of a ``cache`` are of the layer's compute type.  A model that hands caches on to its layers is of that type too: a call converts its
     arguments, and what the layers would then write to is a copy."""
 
